@@ -59,7 +59,7 @@
 extern "C" {
 #endif
 
-#define PA_ABI_VERSION 8
+#define PA_ABI_VERSION 9
 
 /* Return codes. */
 #define PA_OK 0
@@ -327,6 +327,109 @@ int pa_flat_needs_merge(const int32_t *lens, int n, int max_tokens, int flat_spl
  * arguments (the classic split's workspace aside, which may be NULL) as
  * pa_decode does and makes no HIP call. */
 int pa_decode_pairs(const pa_decode_args *args, int *out);
+
+/* Arguments of pa_prefill, pa_diff_prefill and pa_diff_decode. Layouts as for
+ * pa_decode, with the query rows of all sequences packed one after the other:
+ *   q     [num_tokens, num_q_heads, head_dim]                 fp16 | bf16
+ *   out   as q; differential: [num_tokens, num_q_heads / 2, 2 * head_dim]
+ *   query_start_loc [batch + 1] int32, not decreasing: sequence b's rows are
+ *         query_start_loc[b] .. query_start_loc[b + 1] - 1. Rows of no sequence
+ *         (before the first offset, from the last on) are left as they are in out.
+ *   seq_lens [batch]: tokens in the cache, the new ones included
+ *   part_out [num_splits, num_tokens, num_q_heads, head_dim (differential: 2 *
+ *         head_dim)] and part_lse [num_splits, num_tokens, num_q_heads], fp32,
+ *         contiguous: scratch, num_splits > 1 only
+ * Size limits as for pa_decode; num_tokens * num_q_heads below 2^31. */
+typedef struct pa_prefill_args {
+  const void *q;
+  const void *k_cache;
+  const void *v_cache;
+  const void *k_scale; /* int8 only; NULL otherwise */
+  const void *v_scale; /* int8 only; NULL otherwise */
+  void *out;
+  float *part_out; /* num_splits > 1 only; NULL otherwise */
+  float *part_lse; /* num_splits > 1 only; NULL otherwise */
+  const int32_t *block_table;
+  const int32_t *seq_lens;
+  const int32_t *query_start_loc; /* NULL for pa_diff_decode: num_tokens = batch */
+  const float *lam;         /* differential: [num_q_heads / 2], one lambda an output head */
+  const float *norm_weight; /* differential: [2 * head_dim], or NULL for no norm */
+  int32_t batch;
+  int32_t num_tokens;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;   /* 32, 64, 128 or 256; differential: 32, 64 or 128 */
+  int32_t block_size; /* 16, 32, 64, 128 or 256 */
+  int32_t num_blocks; /* pool size; block-table entries are clamped into it */
+  int32_t max_blocks; /* block_table row length */
+  int32_t num_splits; /* >= 1; > 1 cuts every row tile's tokens into that many chunks */
+  int64_t stride_qt, stride_qh;            /* element strides (token, head) */
+  int64_t stride_kn, stride_kt, stride_kh; /* shared by k_cache and v_cache */
+  int64_t stride_sn, stride_st;            /* shared by k_scale and v_scale */
+  int64_t stride_ot, stride_oh;
+  int64_t stride_btb;
+  int64_t stride_lam; /* 0: one lambda for all heads */
+  int32_t kv_dtype;    /* PA_KV_* */
+  int32_t scale_dtype; /* PA_SCALE_* */
+  int32_t io_dtype;    /* PA_IO_* */
+  float sm_scale;      /* positive, finite */
+  float norm_eps;      /* with norm_weight */
+  float out_scale;     /* with norm_weight: factor of the normalised row */
+} pa_prefill_args;
+
+/* Causal paged GQA attention of the last n_b = query_start_loc[b + 1] -
+ * query_start_loc[b] tokens of each sequence over all its T_b = seq_lens[b]
+ * tokens, whose K and V the cache already holds: row i of sequence b sees tokens
+ * 0 .. T_b - n_b + i. A row that sees none (T_b < n_b) yields zeros. */
+int pa_prefill(const pa_prefill_args *args, void *stream);
+
+/* Differential attention of the same rows. Query heads 2 i and 2 i + 1 are the two
+ * maps of output head i; kv heads 2 j and 2 j + 1 are their keys and the two
+ * halves of the value V_j, j = i / (num_q_heads / num_kv_heads):
+ *   o_i = softmax(sm_scale q_2i . K_2j) V_j - lam_i softmax(sm_scale q_2i+1 . K_2j+1) V_j
+ * and with norm_weight o_i = o_i / sqrt(mean(o_i^2) + norm_eps) * norm_weight *
+ * out_scale. A row that sees no token yields zeros. */
+int pa_diff_prefill(const pa_prefill_args *args, void *stream);
+
+/* The same for one new token of each sequence (query_start_loc NULL). */
+int pa_diff_decode(const pa_prefill_args *args, void *stream);
+
+/* Arguments of pa_step_tables. All pointers but finished and positions non-NULL
+ * (those of empty tensors may be). int32 values, contiguous but for the block
+ * table's rows. */
+typedef struct pa_step_tables_args {
+  int32_t *block_table;    /* [batch, max_blocks], changed in place */
+  const int32_t *seq_lens; /* [batch] tokens in the cache before the step */
+  const int32_t *new_lens; /* [batch] tokens that the step adds; <= 0: none */
+  const uint8_t *finished; /* [batch] non-zero: the row's pages return first and it starts
+                              empty; NULL: none */
+  int32_t *free_pages;     /* [free_capacity] stack of free pages; changed only by finished rows */
+  const int32_t *free_count; /* [1] pages on the stack */
+  int32_t *seq_lens_out;   /* [batch] tokens after the step; may be seq_lens */
+  int32_t *free_count_out; /* [1]; may be free_count */
+  int32_t *query_start_loc; /* [batch + 1] first packed token of each row, and the end */
+  int64_t *slot_mapping;   /* [max_tokens] page * block_size + offset; -1 from the end on */
+  int64_t *positions;      /* [max_tokens] position in the sequence, 0 from the end on; or NULL */
+  int32_t batch;
+  int32_t max_blocks;
+  int32_t block_size;    /* >= 1 */
+  int32_t free_capacity; /* at least the pool's pages, for finished rows to return theirs */
+  int32_t max_tokens;    /* packed tokens that the outputs hold */
+  int64_t stride_btb;
+} pa_step_tables_args;
+
+/* One serving step's tables on the device, no host copy of any length. In order:
+ * finished rows push their pages on the stack (row after row, first page first);
+ * each row's new pages are popped from its top, rows in order, into its block-table
+ * row; the slots, positions, start offsets and lengths follow. A row that does not
+ * fit gets no token, and keeps its length and its pages: one that would pass
+ * max_blocks * block_size tokens; every row asking for tokens from the first on
+ * at which the tokens asked for pass max_tokens; every row needing a page from
+ * the first on at which the pages needed pass the stack. (Its
+ * query_start_loc range is empty, which tells it from one that got its tokens.)
+ * Deterministic. A table row owns its pages: a page shared by two rows would be
+ * returned twice. */
+int pa_step_tables(const pa_step_tables_args *args, void *stream);
 
 /* Message for the last non-zero return on the calling thread ("" if none). */
 const char *pa_last_error(void);

@@ -2,8 +2,9 @@
 
 Public surface of the reference package (ParamThakkar123/paged-decode-attention,
 pagedattn/__init__.py:3-13) restricted to the decode path: shapes, the paged
-cache, the decode entry point and the split heuristic. The reference's fp32
-oracle and dense SDPA baselines are test infrastructure here and live outside
+cache, the decode entry point and the split heuristic. Beyond it, for the same
+cache: attention of prompts (`prefill`), differential attention, and a step's
+tables built on the device (`step_tables`). The reference's fp32 oracle and dense SDPA baselines are test infrastructure here and live outside
 the package (oracle/).
 """
 
@@ -25,6 +26,8 @@ from .hip_decode import (
     short_batch_runs_unsplit,
     split_reduce,
 )
+from .prefill import paged_diff_decode_hip, paged_diff_prefill_hip, paged_prefill_hip
+from .step_tables import StepTables, build_step_tables
 
 __all__ = [
     "LLAMA3_8B", "LLAMA3_70B", "MHA_DEBUG", "QWEN25_05B", "KVDType", "ModelShape",
@@ -33,4 +36,6 @@ __all__ = [
     "paged_decode_hip", "paged_decode_triton", "pick_num_splits", "plan_num_splits",
     "plan_decode", "plan_launch", "LaunchPlan", "short_batch_runs_unsplit", "flat_needs_merge", "flat_splits_for", "flat_waves_per_simd",
     "decode_partials", "split_reduce",
+    "paged_prefill_hip", "paged_diff_prefill_hip", "paged_diff_decode_hip",
+    "build_step_tables", "StepTables",
 ]

@@ -1,7 +1,7 @@
 """ctypes binding of `libpagedattn_hip.so` (declared in include/pagedattn.h).
 
-The structures below mirror `pa_decode_args` / `pa_reduce_args` field for
-field. The library is looked up next to this file (where `build.py` writes
+The structures below mirror the header's (`pa_decode_args`, `pa_reduce_args`,
+`pa_cache_write_args`, `pa_prefill_args`, `pa_step_tables_args`) field for field. The library is looked up next to this file (where `build.py` writes
 it) or at $PAGEDATTN_HIP_LIB. There is no fallback: a missing library raises.
 """
 
@@ -12,7 +12,7 @@ import os
 import pathlib
 import threading
 
-PA_ABI_VERSION = 8
+PA_ABI_VERSION = 9
 
 PA_OK = 0
 PA_ERR_INVALID = -1
@@ -55,6 +55,10 @@ EXPORTED_SYMBOLS = (
     "pa_lens_stats",
     "pa_flat_needs_merge",
     "pa_decode_pairs",
+    "pa_prefill",
+    "pa_diff_prefill",
+    "pa_diff_decode",
+    "pa_step_tables",
     "pa_last_error",
     "pa_abi_version",
 )
@@ -158,6 +162,72 @@ class PaCacheWriteArgs(ctypes.Structure):
     ]
 
 
+class PaPrefillArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp),
+        ("k_cache", _vp),
+        ("v_cache", _vp),
+        ("k_scale", _vp),
+        ("v_scale", _vp),
+        ("out", _vp),
+        ("part_out", _vp),
+        ("part_lse", _vp),
+        ("block_table", _vp),
+        ("seq_lens", _vp),
+        ("query_start_loc", _vp),
+        ("lam", _vp),
+        ("norm_weight", _vp),
+        ("batch", _i32),
+        ("num_tokens", _i32),
+        ("num_q_heads", _i32),
+        ("num_kv_heads", _i32),
+        ("head_dim", _i32),
+        ("block_size", _i32),
+        ("num_blocks", _i32),
+        ("max_blocks", _i32),
+        ("num_splits", _i32),
+        ("stride_qt", _i64),
+        ("stride_qh", _i64),
+        ("stride_kn", _i64),
+        ("stride_kt", _i64),
+        ("stride_kh", _i64),
+        ("stride_sn", _i64),
+        ("stride_st", _i64),
+        ("stride_ot", _i64),
+        ("stride_oh", _i64),
+        ("stride_btb", _i64),
+        ("stride_lam", _i64),
+        ("kv_dtype", _i32),
+        ("scale_dtype", _i32),
+        ("io_dtype", _i32),
+        ("sm_scale", ctypes.c_float),
+        ("norm_eps", ctypes.c_float),
+        ("out_scale", ctypes.c_float),
+    ]
+
+
+class PaStepTablesArgs(ctypes.Structure):
+    _fields_ = [
+        ("block_table", _vp),
+        ("seq_lens", _vp),
+        ("new_lens", _vp),
+        ("finished", _vp),
+        ("free_pages", _vp),
+        ("free_count", _vp),
+        ("seq_lens_out", _vp),
+        ("free_count_out", _vp),
+        ("query_start_loc", _vp),
+        ("slot_mapping", _vp),
+        ("positions", _vp),
+        ("batch", _i32),
+        ("max_blocks", _i32),
+        ("block_size", _i32),
+        ("free_capacity", _i32),
+        ("max_tokens", _i32),
+        ("stride_btb", _i64),
+    ]
+
+
 class HipLibraryMissing(ImportError):
     """The HIP library has not been built (run __graft_entry__.build())."""
 
@@ -211,6 +281,11 @@ def load() -> ctypes.CDLL:
         lib.pa_flat_needs_merge.restype = ctypes.c_int
         lib.pa_decode_pairs.argtypes = [ctypes.POINTER(PaDecodeArgs), _vp]
         lib.pa_decode_pairs.restype = ctypes.c_int
+        for fn in (lib.pa_prefill, lib.pa_diff_prefill, lib.pa_diff_decode):
+            fn.argtypes = [ctypes.POINTER(PaPrefillArgs), _vp]
+            fn.restype = ctypes.c_int
+        lib.pa_step_tables.argtypes = [ctypes.POINTER(PaStepTablesArgs), _vp]
+        lib.pa_step_tables.restype = ctypes.c_int
         lib.pa_last_error.argtypes = []
         lib.pa_last_error.restype = ctypes.c_char_p
         lib.pa_abi_version.argtypes = []

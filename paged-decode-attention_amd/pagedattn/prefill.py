@@ -1,0 +1,204 @@
+"""Attention of prompts over the paged cache, and differential attention (HIP).
+
+`paged_prefill_hip` attends several new tokens of each sequence over the cache
+that already holds them (write them with `reshape_and_cache` first): prompts,
+chunks of prompts, a few speculative tokens. `paged_diff_prefill_hip` and
+`paged_diff_decode_hip` are the differential forms, for several tokens and for
+one. Launches go through the C ABI (include/pagedattn.h); there is no CPU path.
+Split partials are allocated per call from torch's caching allocator, on the
+current stream, so calls on different streams and captured graphs share nothing.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _abi
+from .cache import PagedKVCache
+from .hip_decode import _IO_CODE, _KV_CODE, _SCALE_CODE, _STORE_DTYPE, _cu_count, _launch
+
+# Tokens of a kernel tile (csrc/paged_prefill.hip) and rows of a workgroup, by the
+# width of a cache row (a pair of heads for the differential forms).
+ROWS_PER_WORKGROUP = 128
+# Workgroups that a CU holds at once, and the fewest tokens worth a split.
+WORKGROUPS_PER_CU = 2
+MIN_SPLIT_TOKENS = 256
+
+
+def _plan_splits(row_tiles: int, units: int, longest: int, cus: int) -> int:
+    """How many chunks each row tile's tokens are cut into: enough workgroups
+    for the chip, none below MIN_SPLIT_TOKENS tokens."""
+    work = max(1, row_tiles * units)
+    want = WORKGROUPS_PER_CU * cus // work
+    return max(1, min(want, -(-longest // MIN_SPLIT_TOKENS), _abi.PA_MAX_SPLITS))
+
+
+def _attend(fn_name, maps, q, cache, start, out, sm_scale, num_splits, max_seq_len, lam=None, norm_weight=None,
+            norm_eps=0.0, out_scale=1.0):
+    """Validate a call's tensors, pack pa_prefill_args and launch."""
+    if q.dim() != 3:
+        raise ValueError(f"q {tuple(q.shape)} is not [tokens, heads, head_dim]")
+    n, hq, d = q.shape
+    shape, kv_dtype = cache.shape, cache.kv_dtype
+    hkv = shape.num_kv_heads
+    if kv_dtype not in _KV_CODE:
+        raise NotImplementedError(f"kv_dtype {kv_dtype!r} is not supported by the HIP kernel")
+    if q.dtype not in _IO_CODE:
+        raise NotImplementedError(f"q dtype {q.dtype}: float16 or bfloat16")
+    if hq != shape.num_q_heads or d != shape.head_dim:
+        raise ValueError(f"q has {hq} heads of {d}, cache shape expects {shape.num_q_heads} of {shape.head_dim}")
+    if hkv <= 0 or hq % hkv or hkv % maps:
+        raise ValueError(f"{hq} query heads and {hkv} kv heads do not group" + (" in pairs" if maps == 2 else ""))
+    if not q.is_cuda:
+        raise ValueError(f"q is on {q.device}: the HIP kernel needs GPU tensors")
+    k, v, bt, sl = cache.k_cache, cache.v_cache, cache.block_table, cache.seq_lens
+    out_shape = (n, hq // maps, maps * d)
+    if out is None:
+        out = torch.empty(out_shape, dtype=q.dtype, device=q.device)
+    elif out.shape != out_shape or out.dtype != q.dtype:
+        raise ValueError(f"out {out.dtype} {tuple(out.shape)} is not {q.dtype} {out_shape}")
+    dev = q.get_device()
+    for name, t in (("k_cache", k), ("v_cache", v), ("out", out), ("block_table", bt), ("seq_lens", sl),
+                    ("query_start_loc", start), ("lam", lam), ("norm_weight", norm_weight)):
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name} is on {t.device}, q on {q.device}")
+    if k.dtype != _STORE_DTYPE[kv_dtype] or v.dtype != k.dtype:
+        raise ValueError(f"k/v cache dtype {k.dtype}/{v.dtype} does not match kv_dtype {kv_dtype}")
+    kst, qst, ost = k.stride(), q.stride(), out.stride()
+    if tuple(k.shape[1:]) != (cache.block_size, hkv, d) or v.shape != k.shape or v.stride() != kst:
+        raise ValueError(f"k_cache {tuple(k.shape)} is not [NB, {cache.block_size}, {hkv}, {d}], or v_cache differs")
+    if kst[3] != 1 or (qst[2] != 1 and n) or (ost[2] != 1 and n):
+        raise ValueError("head_dim must be the contiguous (stride-1) dimension of q, out and the caches")
+    if bt.dtype != torch.int32 or sl.dtype != torch.int32 or bt.dim() != 2 or sl.dim() != 1:
+        raise ValueError("block_table [B, max_blocks] and seq_lens [B] must be int32")
+    b, blocks = bt.shape
+    if sl.shape[0] != b or (b > 1 and sl.stride(0) != 1) or (blocks > 1 and bt.stride(1) != 1):
+        raise ValueError(f"block_table {tuple(bt.shape)} / seq_lens {tuple(sl.shape)}: [B, n] and [B], rows contiguous")
+    if start is None:
+        if n != b:
+            raise ValueError(f"q has {n} rows for {b} sequences")
+    elif start.dtype != torch.int32 or start.shape != (b + 1,) or (b and start.stride(0) != 1):
+        raise ValueError(f"query_start_loc must be contiguous int32 [{b + 1}]")
+    ks = vs = None
+    sst, scale_code = (0, 0), _abi.PA_SCALE_NONE
+    if kv_dtype == "int8":
+        ks, vs = cache.k_scale, cache.v_scale
+        if ks is None or vs is None or ks.dtype not in _SCALE_CODE or vs.dtype != ks.dtype:
+            raise ValueError("int8 cache needs float16 or float32 k_scale/v_scale")
+        sst = ks.stride()
+        if ks.shape != k.shape[:3] or vs.shape != ks.shape or vs.stride() != sst or sst[2] != 1:
+            raise ValueError("k_scale/v_scale must be [NB, block_size, H_kv] with equal strides and a contiguous "
+                             "head dimension")
+        if ks.get_device() != dev or vs.get_device() != dev:
+            raise ValueError("scales must live on q's device")
+        scale_code, ks, vs = _SCALE_CODE[ks.dtype], ks.data_ptr(), vs.data_ptr()
+    lam_stride = 0
+    if maps == 2:
+        if lam.dtype != torch.float32 or lam.shape != (hq // 2,):
+            raise ValueError(f"lam must be float32 [{hq // 2}], got {lam.dtype} {tuple(lam.shape)}")
+        lam_stride = lam.stride(0)
+        if norm_weight is not None and (norm_weight.dtype != torch.float32 or norm_weight.shape != (2 * d,)
+                                        or norm_weight.stride(0) != 1):
+            raise ValueError(f"norm_weight must be contiguous float32 [{2 * d}]")
+    if n == 0 or b == 0:
+        return out
+    group = hq // hkv
+    if num_splits is None:
+        longest = blocks * cache.block_size if max_seq_len is None else min(int(max_seq_len), blocks * cache.block_size)
+        rows = ROWS_PER_WORKGROUP // maps
+        tiles = b * -(-group // rows) if start is None else max(b, n * group // rows + b // 2)
+        num_splits = _plan_splits(tiles, hkv // maps, longest, _cu_count(q.device))
+    num_splits = int(num_splits)
+    po = pl = None
+    if num_splits > 1:
+        part = torch.empty((num_splits * n * hq * (maps * d + 1),), dtype=torch.float32, device=q.device)
+        po = part.data_ptr()
+        pl = po + 4 * num_splits * n * hq * maps * d
+    args = _abi.PaPrefillArgs(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), ks, vs, out.data_ptr(), po, pl, bt.data_ptr(), sl.data_ptr(),
+        None if start is None else start.data_ptr(), None if lam is None else lam.data_ptr(),
+        None if norm_weight is None else norm_weight.data_ptr(),
+        b, n, hq, hkv, d, cache.block_size, k.shape[0], blocks, num_splits,
+        qst[0], qst[1], kst[0], kst[1], kst[2], sst[0], sst[1], ost[0], ost[1],
+        bt.stride(0) if b > 1 else blocks, lam_stride,
+        _KV_CODE[kv_dtype], scale_code, _IO_CODE[q.dtype], d ** -0.5 if sm_scale is None else float(sm_scale),
+        float(norm_eps), float(out_scale))
+    rc = _launch(q, getattr(_abi.load(), fn_name), args)
+    if rc:
+        _abi.check(rc, fn_name)
+    return out
+
+
+def paged_prefill_hip(
+    q: torch.Tensor,
+    cache: PagedKVCache,
+    query_start_loc: torch.Tensor,
+    out: torch.Tensor | None = None,
+    sm_scale: float | None = None,
+    num_splits: int | None = None,
+    max_seq_len: int | None = None,
+) -> torch.Tensor:
+    """Causal paged GQA attention of several new tokens of each sequence.
+
+    q [tokens, Hq, D] fp16 or bf16 holds the sequences' new tokens packed one
+    sequence after the other: sequence b's are rows query_start_loc[b] ..
+    query_start_loc[b + 1] - 1 (int32 [B + 1] on the device, not decreasing).
+    cache.seq_lens counts the tokens in the cache, the new ones included, so
+    row i of n_b sees tokens 0 .. T_b - n_b + i. A row that sees none is zeros.
+    Rows of no sequence (padding behind the last) are left as they are in `out`.
+
+    `num_splits` cuts each row tile's tokens into that many chunks, joined by a
+    second kernel; None plans it from the shapes alone, with no device sync, by
+    `max_seq_len` (a host int; None: what the block table can hold).
+    """
+    return _attend("pa_prefill", 1, q, cache, query_start_loc, out, sm_scale, num_splits, max_seq_len)
+
+
+def paged_diff_prefill_hip(
+    q: torch.Tensor,
+    cache: PagedKVCache,
+    query_start_loc: torch.Tensor,
+    lam: torch.Tensor,
+    out: torch.Tensor | None = None,
+    norm_weight: torch.Tensor | None = None,
+    norm_eps: float = 1e-5,
+    out_scale: float = 1.0,
+    sm_scale: float | None = None,
+    num_splits: int | None = None,
+    max_seq_len: int | None = None,
+) -> torch.Tensor:
+    """Differential attention of several new tokens of each sequence.
+
+    Heads come in pairs: query heads 2i and 2i + 1 of q [tokens, Hq, D] are the
+    two maps of output head i, kv heads 2j and 2j + 1 of the cache (j = i //
+    group) the keys of the maps and the two halves of the value:
+        out[:, i] = softmax(q_2i K_2j) V_j - lam[i] * softmax(q_2i+1 K_2j+1) V_j
+    out is [tokens, Hq / 2, 2 D]. `lam` float32 [Hq / 2] (one for the layer:
+    `lam.expand(Hq // 2)`). With `norm_weight` float32 [2 D] each head's row is
+    normalised by its root mean square (plus norm_eps) and scaled by norm_weight
+    * out_scale. Rows and the other arguments as in `paged_prefill_hip`.
+    """
+    return _attend("pa_diff_prefill", 2, q, cache, query_start_loc, out, sm_scale, num_splits, max_seq_len, lam,
+                   norm_weight, norm_eps, out_scale)
+
+
+def paged_diff_decode_hip(
+    q: torch.Tensor,
+    cache: PagedKVCache,
+    lam: torch.Tensor,
+    out: torch.Tensor | None = None,
+    norm_weight: torch.Tensor | None = None,
+    norm_eps: float = 1e-5,
+    out_scale: float = 1.0,
+    sm_scale: float | None = None,
+    num_splits: int | None = None,
+    max_seq_len: int | None = None,
+) -> torch.Tensor:
+    """Differential attention of one new token of each sequence: q [B, Hq, D] ->
+    [B, Hq / 2, 2 D]. Arguments as in `paged_diff_prefill_hip`; a sequence of
+    length 0 yields zeros."""
+    return _attend("pa_diff_decode", 2, q, cache, None, out, sm_scale, num_splits, max_seq_len, lam, norm_weight,
+                   norm_eps, out_scale)
+
+
+__all__ = ["paged_prefill_hip", "paged_diff_prefill_hip", "paged_diff_decode_hip"]
