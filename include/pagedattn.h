@@ -340,6 +340,8 @@ int pa_decode_pairs(const pa_decode_args *args, int *out);
  *         head_dim)] and part_lse [num_splits, num_tokens, num_q_heads], fp32,
  *         contiguous: scratch, num_splits > 1 only
  * Size limits as for pa_decode; num_tokens * num_q_heads below 2^31. */
+#define PA_FORM_TILES 0   /* 128 rows (64 differential) a workgroup: many rows a sequence */
+#define PA_FORM_STREAMS 1 /* 32 rows (16 differential): few rows a sequence, any number is right */
 typedef struct pa_prefill_args {
   const void *q;
   const void *k_cache;
@@ -362,7 +364,10 @@ typedef struct pa_prefill_args {
   int32_t block_size; /* 16, 32, 64, 128 or 256 */
   int32_t num_blocks; /* pool size; block-table entries are clamped into it */
   int32_t max_blocks; /* block_table row length */
-  int32_t num_splits; /* >= 1; > 1 cuts every row tile's tokens into that many chunks */
+  int32_t num_splits; /* >= 1; > 1 cuts every row tile's tokens into at most that many chunks */
+  int32_t max_seq_len; /* > 0: chunks no shorter than those of a sequence this long, so a
+                          ragged batch's short sequences take few; 0: each its own */
+  int32_t form;        /* PA_FORM_* */
   int64_t stride_qt, stride_qh;            /* element strides (token, head) */
   int64_t stride_kn, stride_kt, stride_kh; /* shared by k_cache and v_cache */
   int64_t stride_sn, stride_st;            /* shared by k_scale and v_scale */

@@ -52,6 +52,7 @@ typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 constexpr int kWaves = 4;
 constexpr int kRowsPerWave = 32;
 constexpr float kRescaleLog2 = 8.0f;
+constexpr int kSplitUnit = 128;  // splits are multiples of this many tokens
 // A lane offset past every buffer (page_rsrc's -1 leaves all others in range):
 // the load returns zeros.
 constexpr uint32_t kOutside = 0xfffffff0u;
@@ -73,6 +74,7 @@ struct PParams {
   const float *norm;     // differential: [DV] or NULL
   int32_t batch, num_tokens, units, group, num_q_heads;
   int32_t num_blocks, max_tokens, log2_page, num_splits;
+  int32_t max_seq_len;   // > 0: chunks no shorter than those of a sequence this long
   int32_t tiles;         // row tiles of the launch
   int32_t sqt, sqh, sot, soh;  // elements
   uint32_t skn, skt, skh, ssn, sst;  // bytes
@@ -170,11 +172,13 @@ __device__ __forceinline__ RowTile tile_at(const PParams &p, int b, int index) {
   return t;
 }
 
-// Token range of a split of `hi` tokens, whole tiles of BN each (empty: lo >= hi).
-template <int BN>
+// Tokens of a split of a row tile that sees `hi`, a multiple of UNIT: the tile's own
+// chunk, or that of a tile that sees max_seq_len if it is larger (ragged batches:
+// long sequences take all splits, short ones few).
+template <int UNIT>
 __device__ __forceinline__ int split_tokens(const PParams &p, int hi) {
-  const uint32_t tiles = ((uint32_t)hi + BN - 1) / BN;
-  return (int)div_by(tiles + p.num_splits - 1, p.by_splits) * BN;
+  const uint32_t units = ((uint32_t)max(hi, p.max_seq_len) + UNIT - 1) / UNIT;
+  return (int)div_by(units + p.num_splits - 1, p.by_splits) * UNIT;
 }
 
 template <int KV, int SC, int D, int MAPS>
@@ -300,6 +304,14 @@ __device__ __forceinline__ bool has_wild(uint32_t w) {
   return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
 }
 
+// Infinities and NaN of the word's halves to zeros; whether there was one.
+__device__ __forceinline__ bool tame_word(uint32_t &w) {
+  if (__builtin_expect(!has_wild(w), 1)) return false;
+  if ((w & 0x7c00u) == 0x7c00u) w &= 0xffff0000u;
+  if ((w & 0x7c000000u) == 0x7c000000u) w &= 0xffffu;
+  return true;
+}
+
 // The staged tile into an LDS buffer (K rows, then V rows). With `tame`,
 // infinities and NaN of V become zeros, and the result tells whether this lane
 // had one.
@@ -319,12 +331,7 @@ __device__ __forceinline__ bool store_tile(uint8_t *buf, const Staged<KV, SC, D,
     to_halves<KV, SC>(h, st.v[i], KV == PA_KV_INT8 ? st.vs[KV == PA_KV_INT8 ? i : 0] : 0);
     if (tame) {
 #pragma unroll
-      for (int w = 0; w < kHalves; ++w)
-        if (__builtin_expect(has_wild(h[w]), 0)) {
-          wild = true;
-          if ((h[w] & 0x7c00u) == 0x7c00u) h[w] &= 0xffff0000u;
-          if ((h[w] & 0x7c000000u) == 0x7c000000u) h[w] &= 0xffffu;
-        }
+      for (int w = 0; w < kHalves; ++w) wild |= tame_word(h[w]);
     }
     uint8_t *vd = buf + G::kKBytes + la.row[i] * G::kVStride + col * 2;
 #pragma unroll
@@ -354,51 +361,60 @@ struct RowState {
   float l;  // sum over this lane's tokens
 };
 
-// One tile of BN tokens from n0 on. `masked`: some row of the wave does not see
-// all of them (`lim` is the last token that this lane's row sees).
-template <int KV, int D, int MAPS>
-__device__ __forceinline__ void compute_tile(RowState<D, D * MAPS> &st, const uint8_t *buf, float qk_scale, int n0,
-                                             int lim, bool masked, int map, int lane) {
-  using G = PGeo<KV, D, MAPS>;
-  constexpr int NB = G::BN / 32;
-  const int col = lane & 31, h = lane >> 5;
-  const uint8_t *krow = buf + col * G::kKStride + map * D * 2 + 16 * h;
-  const uint8_t *v = buf + G::kKBytes;
-  const uint32_t v_lane = (4 * h + ((lane & 15) >> 2)) * G::kVStride + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-
-  f32x16 s[NB];
+// Scores of a tile's tokens: lane (row = lane & 31, half h) holds those of tokens
+// 32 b + 8 (i / 4) + 4 h + i % 4 in s[b][i]. `k`: this lane's K operand in LDS.
+template <int KSTEPS, int STRIDE, int NB>
+__device__ __forceinline__ void scores_of(f32x16 (&s)[NB], const f16x8 *q, const uint8_t *k) {
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     s[b] = f32x16{};
 #pragma unroll
-    for (int ks = 0; ks < G::kKSteps; ++ks) {
-      const f16x8 kop = *reinterpret_cast<const f16x8 *>(krow + 32 * b * G::kKStride + 32 * ks);
-      s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kop, st.q[ks], s[b], 0, 0, 0);
+    for (int ks = 0; ks < KSTEPS; ++ks) {
+      const f16x8 kop = *reinterpret_cast<const f16x8 *>(k + 32 * b * STRIDE + 32 * ks);
+      s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kop, q[ks], s[b], 0, 0, 0);
     }
   }
-  if (masked) {
+}
+
+// Scores of tokens that the lane's row does not see (past `lim`) become -inf.
+template <int NB>
+__device__ __forceinline__ void mask(f32x16 (&s)[NB], int n0, int lim, int h) {
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (n0 + 32 * b + 8 * (i / 4) + 4 * h + i % 4 > lim) s[b][i] = -INFINITY;
-  }
+    for (int i = 0; i < 16; ++i)
+      if (n0 + 32 * b + 8 * (i / 4) + 4 * h + i % 4 > lim) s[b][i] = -INFINITY;
+}
+
+// The largest score of the lane's row, in the log2 domain.
+template <int NB>
+__device__ __forceinline__ float top_score(const f32x16 (&s)[NB], float qk_scale) {
   float top = s[0][0];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-  top = half_max(top) * qk_scale;
+  return half_max(top) * qk_scale;
+}
 
+// Moves the running maximum to `top` where that is far above it.
+template <int D, int W>
+__device__ __forceinline__ void rescale(RowState<D, W> &st, float top) {
   const bool need = top > st.m + kRescaleLog2;
   if (__builtin_expect(__builtin_amdgcn_ballot_w64(need) != 0, 0)) {
     const float m_new = need ? top : st.m;
     const float alpha = need ? __builtin_amdgcn_exp2f(st.m - m_new) : 1.0f;
     st.l *= alpha;
 #pragma unroll
-    for (int d = 0; d < G::kDB; ++d) st.acc[d] *= alpha;
+    for (int d = 0; d < W / 32; ++d) st.acc[d] *= alpha;
     st.m = m_new;
   }
+}
+
+// Scores to P, and O^T += V^T P^T.
+template <int VSTRIDE, int D, int W, int NB>
+__device__ __forceinline__ void accumulate(RowState<D, W> &st, f32x16 (&s)[NB], const uint8_t *v, uint32_t v_lane,
+                                           float qk_scale) {
   // (a row that has seen nothing yet: every score is -inf and P is 0)
   const float m = st.m == -INFINITY ? 0.f : st.m;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -410,30 +426,31 @@ __device__ __forceinline__ void compute_tile(RowState<D, D * MAPS> &st, const ui
       sum[i & 3] += s[b][i];
     }
   st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-
 #pragma unroll
-  for (int kb = 0; kb < G::BN / 16; ++kb) {
+  for (int kb = 0; kb < 2 * NB; ++kb) {
     uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = cvt_pk_f16(s[kb / 2][8 * (kb & 1) + 2 * j], s[kb / 2][8 * (kb & 1) + 2 * j + 1]);
+    for (int j = 0; j < 4; ++j) {
+      const f16x2 two = {(_Float16)s[kb / 2][8 * (kb & 1) + 2 * j], (_Float16)s[kb / 2][8 * (kb & 1) + 2 * j + 1]};
+      w[j] = __builtin_bit_cast(uint32_t, two);
+    }
     const f16x8 pop = as_f16x8(w[0], w[1], w[2], w[3]);
 #pragma unroll
-    for (int d = 0; d < G::kDB; ++d)
-      st.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(read_v<G::kVStride>(v, kb, d, v_lane), pop, st.acc[d], 0, 0, 0);
+    for (int d = 0; d < W / 32; ++d)
+      st.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(read_v<VSTRIDE>(v, kb, d, v_lane), pop, st.acc[d], 0, 0, 0);
   }
 }
 
 // The infinities and NaN of V in a masked tile. A product with P = 0 would hand
-// them to rows that do not see their token, so compute_tile had zeros in their
+// them to rows that do not see their token, so the tile had zeros in their
 // place; here they are added to the rows that see them, as they are: whatever P
 // above zero they meet, the sum is what it would be.
-template <int KV, int D, int MAPS>
-__device__ __forceinline__ void add_wild(RowState<D, D * MAPS> &st, const uint8_t *buf, int n0, int lim, int lane) {
-  using G = PGeo<KV, D, MAPS>;
-  for (int t = 0; t < G::BN; ++t) {
-    const uint8_t *row = buf + G::kKBytes + t * G::kVStride + 8 * (lane >> 5);
+template <int BN, int VSTRIDE, int D, int W>
+__device__ __forceinline__ void add_wild(RowState<D, W> &st, const uint8_t *v, int n0, int lim, int lane) {
+  for (int t = 0; t < BN; ++t) {
+    const uint8_t *row = v + t * VSTRIDE + 8 * (lane >> 5);
 #pragma unroll
-    for (int d = 0; d < G::kDB; ++d)
+    for (int d = 0; d < W / 32; ++d)
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         const u32x2 w = *reinterpret_cast<const u32x2 *>(row + 64 * d + 4 * i);
@@ -457,6 +474,40 @@ __device__ __forceinline__ void store4(uint8_t *dst, float a, float b, float c, 
     w = u32x2{cvt_pk_f16(a, b), cvt_pk_f16(c, d)};
   }
   *reinterpret_cast<u32x2 *>(dst) = w;
+}
+
+// A lane's accumulators (elements 32 d + 2 i + 4 h .. + 3 in acc[d][i .. i + 3], i a
+// multiple of 4) as an output row: times f, and with `normed` times the norm's
+// weight if there is one.
+template <int W>
+__device__ __forceinline__ void store_rows(const PParams &p, const f32x16 *acc, float f, bool normed, int packed,
+                                           int out_head, int h) {
+  uint8_t *dst = p.out + 2 * ((int64_t)packed * p.sot + (int64_t)out_head * p.soh + 4 * h);
+  const float *norm = normed ? p.norm : nullptr;
+#pragma unroll
+  for (int d = 0; d < W / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      f32x4 y = {acc[d][i] * f, acc[d][i + 1] * f, acc[d][i + 2] * f, acc[d][i + 3] * f};
+      if (norm) y *= *reinterpret_cast<const f32x4 *>(norm + 32 * d + 2 * i + 4 * h);
+      store4(dst + 2 * (32 * d + 2 * i), y.x, y.y, y.z, y.w, p.io_bf16);
+    }
+}
+
+// The same as a partial: normalised, and its log2-sum-exp.
+template <int W>
+__device__ __forceinline__ void store_partial(const PParams &p, const f32x16 *acc, float m, float l, int split,
+                                              int packed, int head, int h) {
+  const int64_t at = ((int64_t)split * p.num_tokens + packed) * p.num_q_heads + head;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  float *dst = p.part_out + at * W + 4 * h;
+#pragma unroll
+  for (int d = 0; d < W / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      *reinterpret_cast<f32x4 *>(dst + 32 * d + 2 * i) =
+          f32x4{acc[d][i] * inv, acc[d][i + 1] * inv, acc[d][i + 2] * inv, acc[d][i + 3] * inv};
+  if (h == 0) p.part_lse[at] = l == 0.f ? -INFINITY : m + __log2f(l);
 }
 
 template <int KV, int SC, int D, int MAPS>
@@ -498,11 +549,13 @@ paged_prefill_kernel(const PParams p) {
   if (rt.row0 >= rt.rows) return;
 
   int lo = 0, hi = rt.hi;
+  bool direct = true;  // the row tile is this workgroup's alone: no partials
   if (p.num_splits > 1) {
-    const int chunk = split_tokens<G::BN>(p, rt.hi);
+    const int chunk = split_tokens<kSplitUnit>(p, rt.hi);
+    if (split > 0 && (int64_t)split * chunk >= rt.hi) return;  // empty
     lo = split * chunk;
     hi = min(rt.hi, lo + chunk);
-    if (lo >= hi && split > 0) return;  // (the merge leaves it out; split 0 of a tile that sees nothing is written)
+    direct = rt.hi <= chunk;
   }
 
   // this lane's row: its token, its head, the last token it sees
@@ -559,6 +612,8 @@ paged_prefill_kernel(const PParams p) {
     __syncthreads();  // (sm_wild)
     if (store_tile<KV, SC, D, MAPS>(sm, staged, la, col, lo + G::BN > least_all)) sm_wild = 1;
     __syncthreads();
+    const uint32_t k_lane = (lane & 31) * G::kKStride + map * D * 2 + 16 * h;
+    const uint32_t v_lane = (4 * h + ((lane & 15) >> 2)) * G::kVStride + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
     int cur = 0;
     for (int n0 = lo; n0 < hi; n0 += G::BN) {
       const bool more = n0 + G::BN < hi;
@@ -566,7 +621,15 @@ paged_prefill_kernel(const PParams p) {
         load(n0 + G::BN);
         load_pages<KV, D, MAPS>(page, p, bt_row, n0 + 2 * G::BN, rt.len, wave);
       }
-      compute_tile<KV, D, MAPS>(st, sm + cur * G::kBufBytes, p.qk_scale, n0, lim, n0 + G::BN > least, map, lane);
+      const uint8_t *buf = sm + cur * G::kBufBytes;
+      f32x16 s[G::BN / 32];
+      scores_of<G::kKSteps, G::kKStride>(s, st.q, buf + k_lane);
+      if (n0 + G::BN > least) {
+        asm volatile("");  // a branch: as selects these would run on every tile
+        mask(s, n0, lim, h);
+      }
+      rescale(st, top_score(s, p.qk_scale));
+      accumulate<G::kVStride>(st, s, buf + G::kKBytes, v_lane, p.qk_scale);
       if (more && store_tile<KV, SC, D, MAPS>(sm + (cur ^ 1) * G::kBufBytes, staged, la, col, n0 + 2 * G::BN > least_all))
         sm_wild = 1;
       __syncthreads();
@@ -580,44 +643,26 @@ paged_prefill_kernel(const PParams p) {
         load(n0);
         store_tile<KV, SC, D, MAPS>(sm, staged, la, col, false);
         __syncthreads();
-        if (n0 + G::BN > least_all) add_wild<KV, D, MAPS>(st, sm, n0, lim, lane);
+        if (n0 + G::BN > least_all) add_wild<G::BN, G::kVStride>(st, sm + G::kKBytes, n0, lim, lane);
         __syncthreads();
       }
     }
   }
 
   const float l = half_sum(st.l);
-  if (p.num_splits > 1) {
-    if (!live) return;
-    const int64_t at = ((int64_t)split * p.num_tokens + rt.token0 + token) * p.num_q_heads + head;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    float *dst = p.part_out + at * W + 4 * h;
-#pragma unroll
-    for (int d = 0; d < G::kDB; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        *reinterpret_cast<f32x4 *>(dst + 32 * d + 2 * i) =
-            f32x4{st.acc[d][i] * inv, st.acc[d][i + 1] * inv, st.acc[d][i + 2] * inv, st.acc[d][i + 3] * inv};
-    if (h == 0) p.part_lse[at] = l == 0.f ? -INFINITY : st.m + __log2f(l);
+  if (!direct) {
+    if (live) store_partial<W>(p, st.acc, st.m, l, split, rt.token0 + token, head, h);
     return;
   }
   // (a row that sees nothing is zeros; one whose visible scores are all -inf is 0 / 0)
   float inv = lim < 0 ? 0.f : 1.0f / l;
-  const int out_head = head / MAPS;
-  uint8_t *dst = p.out + 2 * ((int64_t)(rt.token0 + token) * p.sot + (int64_t)out_head * p.soh + 4 * h);
   if constexpr (MAPS == 1) {
-    if (!live) return;
-#pragma unroll
-    for (int d = 0; d < G::kDB; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        store4(dst + 2 * (32 * d + 2 * i), st.acc[d][i] * inv, st.acc[d][i + 1] * inv, st.acc[d][i + 2] * inv,
-               st.acc[d][i + 3] * inv, p.io_bf16);
+    if (live) store_rows<W>(p, st.acc, inv, false, rt.token0 + token, head, h);
   } else {
     float *other = reinterpret_cast<float *>(sm) + (wave / 2) * (W / 2) * 64;
     __syncthreads();  // every wave is done with the tiles
     if (map == 1) {
-      inv *= p.lam[(int64_t)out_head * p.slam];
+      inv *= p.lam[(int64_t)(head / 2) * p.slam];
 #pragma unroll
       for (int d = 0; d < G::kDB; ++d)
 #pragma unroll
@@ -636,23 +681,322 @@ paged_prefill_kernel(const PParams p) {
     sq = half_sum(sq);
     if (!live) return;
     const float f = p.norm ? __builtin_amdgcn_rsqf(sq * (1.0f / W) + p.norm_eps) * p.out_scale : 1.0f;
+    store_rows<W>(p, st.acc, f, true, rt.token0 + token, head / 2, h);
+  }
+}
+
+// ----------------------------------------------------------------------------
+// Few rows: 32 columns of S^T hold all rows of a (sequence, kv head), or of 16 of
+// its (token, head) pairs with both maps (columns 0-15 and 16-31). Then the four
+// waves of a workgroup share rows, not tokens: wave w takes the 32-token tiles w,
+// w + 4, ... of the workgroup's range, through LDS of its own, with no barrier
+// until the end, where the four are joined as splits are. What bounds it is the
+// stream of K and V: a wave's next tile is in flight while it computes one.
+//
+// The maps of a differential row differ in the half of the K row they meet: each
+// half's products are summed on their own, with q zero in the other map's
+// columns, and a lane keeps its column's sum (what the other half holds,
+// infinities too, stays out of it).
+// ----------------------------------------------------------------------------
+
+template <int KV, int D, int MAPS>
+struct SGeo {
+  static constexpr int W = D * MAPS;
+  static constexpr int kElem = (KV == PA_KV_FP16 || KV == PA_KV_BF16) ? 2 : 1;
+  static constexpr int kPieceBytes = W * kElem >= 64 ? 16 : 8;
+  static constexpr int kPieceElems = kPieceBytes / kElem;
+  static constexpr int kPieceWords = kPieceBytes / 4;
+  static constexpr int kPPR = W / kPieceElems;     // 4 .. 32
+  static constexpr int kIter = 32 * kPPR / 64;     // loads of K (and of V) a tile
+  static constexpr int kKStride = W * 2 + 16;
+  static constexpr int kVStride = W == 32 ? 64 : W * 2 + 64;
+  static constexpr int kSlot = 32 * (kKStride + kVStride);  // LDS of a wave
+  static constexpr int kKSteps = W / 16;
+  static constexpr int kDB = W / 32;
+  static constexpr int kRowTile = 32 / MAPS;
+  static constexpr int kWavesPerEU = W == 256 ? 1 : 2;
+  // Rows of 512 bytes: K and V take turns in the same registers (both at once, with
+  // accumulators and q, do not fit 512); a wave then has 16 KB in flight as others do.
+  static constexpr bool kTurns = W * kElem > 256;
+};
+
+// K or V of a tile on its way to LDS.
+template <int KV, int D, int MAPS>
+struct StreamHalf {
+  using G = SGeo<KV, D, MAPS>;
+  uint32_t w[G::kIter][G::kPieceWords];
+  uint32_t scale[KV == PA_KV_INT8 ? G::kIter : 1];
+};
+
+template <int KV, int SC, int D, int MAPS>
+__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(SGeo<KV, D, MAPS>::kWavesPerEU)))
+paged_stream_kernel(const PParams p) {
+  using G = SGeo<KV, D, MAPS>;
+  constexpr int W = G::W;
+  constexpr int kAccBytes = (kWaves - 1) * (W / 2) * 64 * 4;
+  constexpr int kBytes = kWaves * G::kSlot > kAccBytes ? kWaves * G::kSlot : kAccBytes;
+  __shared__ __attribute__((aligned(16))) uint8_t sm[kBytes];
+  __shared__ float sm_m[kWaves][32], sm_l[kWaves][32];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, h = lane >> 5;
+  const int map = MAPS == 2 ? col >> 4 : 0;
+
+  // blockIdx = (tile * num_splits + split) * units + unit
+  const uint32_t x1 = div_by(blockIdx.x, p.by_units);
+  const int unit = blockIdx.x - x1 * p.units;
+  const uint32_t x2 = div_by(x1, p.by_splits);
+  const int split = x1 - x2 * p.num_splits;
+  const int tile = (int)x2;
+  int b, index;
+  if (p.start) {
+    auto key = [&](int start, int seq) { return (int)((uint32_t)(start * p.group) / G::kRowTile) + seq; };
+    b = find_sequence(p, tile, lane, key);
+    index = tile - key(row_start(p, b), b);
+    if (index < 0) return;
+  } else {
+    b = div_by(tile, p.by_seq_tiles);
+    index = tile - b * p.by_seq_tiles.d;
+  }
+  const RowTile rt = tile_at<G::kRowTile>(p, b, index);
+  if (rt.row0 >= rt.rows) return;
+  int lo = 0, hi = rt.hi;
+  bool direct = true;
+  if (p.num_splits > 1) {
+    const int chunk = split_tokens<kSplitUnit>(p, rt.hi);
+    if (split > 0 && (int64_t)split * chunk >= rt.hi) return;
+    lo = split * chunk;
+    hi = min(rt.hi, lo + chunk);
+    direct = rt.hi <= chunk;
+  }
+
+  const int row = rt.row0 + (MAPS == 2 ? col & 15 : col);
+  const bool live = row < rt.rows;
+  const int r = min(row, rt.rows - 1);
+  const int token = div_by((uint32_t)r, p.by_group);
+  const int head = MAPS * (unit * p.group + (r - token * p.group)) + map;
+  const int lim = rt.first + token;
+  const int least = rt.first + (int)div_by((uint32_t)rt.row0, p.by_group) + 1;  // tokens that the first row sees
+
+  RowState<W, W> st;
+  st.m = -INFINITY;
+  st.l = 0.f;
+#pragma unroll
+  for (int d = 0; d < G::kDB; ++d) st.acc[d] = f32x16{};
+  {
+    const uint16_t *qrow = reinterpret_cast<const uint16_t *>(p.q) + (int64_t)(rt.token0 + token) * p.sqt +
+                           (int64_t)head * p.sqh + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const u32x4 w = *reinterpret_cast<const u32x4 *>(qrow + 16 * ks);
+      const f16x8 x = p.io_bf16 ? bf16x8_to_f16x8(w) : __builtin_bit_cast(f16x8, w);
+      if constexpr (MAPS == 1) {
+        st.q[ks] = x;
+      } else {
+        st.q[ks] = map == 0 ? x : f16x8{};
+        st.q[D / 16 + ks] = map == 1 ? x : f16x8{};
+      }
+    }
+  }
+
+  // this lane's piece of a load: row (of 64 / kPPR), element
+  const int row_in = lane / G::kPPR;
+  const int ecol = lane % G::kPPR * G::kPieceElems;
+  const uint32_t part = (uint32_t)ecol / D;
+  const uint32_t off = row_in * p.skt + part * p.skh + ((uint32_t)ecol - part * D) * G::kElem;
+  const uint32_t soff = row_in * p.sst + part * (SC == PA_SCALE_FP32 ? 4 : 2);
+  const int64_t head_off = (int64_t)unit * MAPS * p.skh;
+  const int64_t scale_off = (int64_t)unit * MAPS * (SC == PA_SCALE_FP32 ? 4 : 2);
+  const ro_i32 *bt_row = ro(p.bt) + (int64_t)rt.b * p.sbtb;
+  uint8_t *slot = sm + wave * G::kSlot;
+
+  // tile at n0 (a multiple of 32: a 16-token half lies in one page)
+  auto pages = [&](int n0, int (&pg)[2]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) pg[u] = bt_row[(uint32_t)min(n0 + 16 * u, rt.len - 1) >> p.log2_page];
+  };
+  StreamHalf<KV, D, MAPS> first_half, second_half;
+  auto &tk = first_half;
+  auto &tv = G::kTurns ? first_half : second_half;
+  auto load = [&](StreamHalf<KV, D, MAPS> &t, const uint8_t *base, const uint8_t *sbase, int n0, const int (&pg)[2]) {
+#pragma unroll
+    for (int i = 0; i < G::kIter; ++i) {
+      const int r0 = i * (64 / G::kPPR);  // first row of the load
+      const uint32_t blk = (uint32_t)min(max(pg[r0 / 16], 0), p.num_blocks - 1);
+      const uint32_t in_page = (uint32_t)(n0 + r0) & ((1u << p.log2_page) - 1u);
+      const bool inside = n0 + r0 + row_in < rt.len;
+      load_piece(t.w[i], page_rsrc(base + head_off + (uint64_t)blk * p.skn + in_page * p.skt, kRsrcBytes),
+                 inside ? off : kOutside);
+      if constexpr (KV == PA_KV_INT8)
+        t.scale[i] = load_scale<SC>(page_rsrc(sbase + scale_off + (uint64_t)blk * p.ssn + in_page * p.sst, kRsrcBytes),
+                                    inside ? soff : kOutside);
+    }
+  };
+  auto load_k = [&](int n0, const int (&pg)[2]) { load(tk, p.k, p.ks, n0, pg); };
+  auto load_v = [&](int n0, const int (&pg)[2]) { load(tv, p.v, p.vs, n0, pg); };
+  // into the wave's slot; with `tame` as store_tile does for V
+  auto store = [&](const StreamHalf<KV, D, MAPS> &t, uint8_t *dst, int stride, bool tame) {
+    bool wild = false;
+#pragma unroll
+    for (int i = 0; i < G::kIter; ++i) {
+      constexpr int kHalves = G::kPieceElems / 2;
+      uint32_t x[kHalves];
+      to_halves<KV, SC>(x, t.w[i], KV == PA_KV_INT8 ? t.scale[KV == PA_KV_INT8 ? i : 0] : 0);
+      if (tame) {
+#pragma unroll
+        for (int w = 0; w < kHalves; ++w) wild |= tame_word(x[w]);
+      }
+      uint8_t *d = dst + (i * (64 / G::kPPR) + row_in) * stride + ecol * 2;
+#pragma unroll
+      for (int w = 0; w < kHalves; w += 4) *reinterpret_cast<u32x4 *>(d + 4 * w) = u32x4{x[w], x[w + 1], x[w + 2], x[w + 3]};
+    }
+    return wild;
+  };
+  auto store_k = [&] { store(tk, slot, G::kKStride, false); };
+  auto store_v = [&](bool tame) { return store(tv, slot + 32 * G::kKStride, G::kVStride, tame); };
+  auto sync_slot = [] {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+
+  const uint8_t *k_lane = slot + col * G::kKStride + 16 * h;
+  const uint8_t *v_slot = slot + 32 * G::kKStride;
+  const uint32_t v_lane = (4 * h + ((lane & 15) >> 2)) * G::kVStride + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+  const int n_first = lo + 32 * wave;
+  bool wild = false;
+  if (n_first < hi) {
+    int pg[2];
+    pages(n_first, pg);
+    load_k(n_first, pg);
+    if constexpr (G::kTurns) store_k();
+    load_v(n_first, pg);
+    pages(n_first + 32 * kWaves, pg);
+    for (int n0 = n_first; n0 < hi; n0 += 32 * kWaves) {
+      const bool masked = n0 + 32 > least;
+      const int next = n0 + 32 * kWaves;
+      if constexpr (!G::kTurns) {
+        store_k();
+        wild |= store_v(masked);
+      }
+      sync_slot();
+      if (!G::kTurns && next < hi) {
+        load_k(next, pg);
+        load_v(next, pg);
+        pages(next + 32 * kWaves, pg);
+      }
+      f32x16 s[1];
+      if constexpr (MAPS == 1) {
+        scores_of<G::kKSteps, G::kKStride>(s, st.q, k_lane);
+      } else {
+        f32x16 s2[1];
+        scores_of<G::kKSteps / 2, G::kKStride>(s, st.q, k_lane);
+        scores_of<G::kKSteps / 2, G::kKStride>(s2, st.q + G::kKSteps / 2, k_lane + 2 * D);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[0][i] = map == 1 ? s2[0][i] : s[0][i];
+      }
+      if (masked) {
+        asm volatile("");  // a branch
+        mask(s, n0, lim, h);
+      }
+      rescale(st, top_score(s, p.qk_scale));
+      if constexpr (G::kTurns) {
+        wild |= store_v(masked);
+        sync_slot();
+        if (next < hi) load_k(next, pg);
+      }
+      accumulate<G::kVStride>(st, s, v_slot, v_lane, p.qk_scale);
+      sync_slot();
+      if (G::kTurns && next < hi) {
+        store_k();
+        load_v(next, pg);
+        pages(next + 32 * kWaves, pg);
+      }
+    }
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(wild) != 0, 0)) {
+      for (int n0 = n_first; n0 < hi; n0 += 32 * kWaves) {
+        if (n0 + 32 <= least) continue;
+        pages(n0, pg);
+        load_v(n0, pg);
+        store_v(false);
+        sync_slot();
+        add_wild<32, G::kVStride>(st, v_slot, n0, lim, lane);
+        sync_slot();
+      }
+    }
+  }
+
+  // join the waves
+  const float lw = half_sum(st.l);
+  if (h == 0) {
+    sm_m[wave][col] = st.m;
+    sm_l[wave][col] = lw;
+  }
+  __syncthreads();  // (and every wave is done with its slot)
+  float m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, sm_m[w][col]);
+  float l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float mw = sm_m[w][col];
+    // (a wave that saw nothing of the row has a sum of zero)
+    l += mw == -INFINITY ? sm_l[w][col] : sm_l[w][col] * __builtin_amdgcn_exp2f(mw - m);
+  }
+  const float f = st.m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - m);
+  float *others = reinterpret_cast<float *>(sm);
+  if (wave > 0) {
 #pragma unroll
     for (int d = 0; d < G::kDB; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        f32x4 y = {st.acc[d][i] * f, st.acc[d][i + 1] * f, st.acc[d][i + 2] * f, st.acc[d][i + 3] * f};
-        if (p.norm) y *= *reinterpret_cast<const f32x4 *>(p.norm + 32 * d + 2 * i + 4 * h);
-        store4(dst + 2 * (32 * d + 2 * i), y.x, y.y, y.z, y.w, p.io_bf16);
+      for (int i = 0; i < 16; ++i) others[((wave - 1) * (W / 2) + 16 * d + i) * 64 + lane] = st.acc[d][i] * f;
+  }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int d = 0; d < G::kDB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float a = st.acc[d][i] * f;
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) a += others[((w - 1) * (W / 2) + 16 * d + i) * 64 + lane];
+      st.acc[d][i] = a;
+    }
+  if (!direct) {
+    if (live) store_partial<W>(p, st.acc, m, l, split, rt.token0 + token, head, h);
+    return;
+  }
+  float inv = lim < 0 ? 0.f : 1.0f / l;
+  if constexpr (MAPS == 1) {
+    if (live) store_rows<W>(p, st.acc, inv, false, rt.token0 + token, head, h);
+  } else {
+    // columns c and c + 16 (lanes apart by 16) hold the maps of a row
+    if (map == 1) inv *= p.lam[(int64_t)(head / 2) * p.slam];
+    float sq = 0.f;
+#pragma unroll
+    for (int d = 0; d < G::kDB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t x = __float_as_uint(st.acc[d][i] * inv);
+        const auto two = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        const float y = __uint_as_float(two[0]) - __uint_as_float(two[1]);
+        st.acc[d][i] = y;
+        sq += y * y;
       }
+    sq = half_sum(sq);
+    if (live && map == 0) {
+      const float scale = p.norm ? __builtin_amdgcn_rsqf(sq * (1.0f / W) + p.norm_eps) * p.out_scale : 1.0f;
+      store_rows<W>(p, st.acc, scale, true, rt.token0 + token, head / 2, h);
+    }
   }
 }
 
 // Joins the partials of a split launch: one wave an output row, W / 64 elements a
-// lane (W = 32: the upper half of the wave idles). Empty splits were not written
-// and are not read.
-template <int W, int MAPS, int BN>
+// lane (W = 32: the upper half of the wave idles). Row tiles of one split are done;
+// empty splits were not written and are not read.
+template <int W, int MAPS, int ROWS>
 __global__ void __launch_bounds__(256) prefill_merge_kernel(const PParams p) {
-  constexpr int ROWS = kRowsPerWave * kWaves / MAPS;
   constexpr int E = W >= 64 ? W / 64 : 1;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -670,8 +1014,9 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(const PParams p) {
   const int token = packed - row_start(p, b);
   const int in_group = out_head % p.group;
   const RowTile rt = tile_at<ROWS>(p, b, (token * p.group + in_group) / ROWS);
-  const int chunk = split_tokens<BN>(p, rt.hi);
-  const int n = rt.hi > 0 ? (rt.hi + chunk - 1) / chunk : 0;
+  const int chunk = split_tokens<kSplitUnit>(p, rt.hi);
+  if (rt.hi <= chunk) return;  // written by its one workgroup
+  const int n = (rt.hi - 1) / chunk + 1;
   const bool sees = rt.first + token >= 0;
 
   float y[E] = {};
@@ -748,6 +1093,8 @@ int build(const pa_prefill_args *a, int maps, PParams *out) {
     return pa_fail(PA_ERR_INVALID, "num_splits %d not in [1, %d]", a->num_splits, PA_MAX_SPLITS);
   if (a->num_splits > 1 && (!a->part_out || !a->part_lse))
     return pa_fail(PA_ERR_INVALID, "num_splits %d needs part_out and part_lse", a->num_splits);
+  if (a->max_seq_len < 0) return pa_fail(PA_ERR_INVALID, "max_seq_len %d < 0", a->max_seq_len);
+  if (a->form != PA_FORM_TILES && a->form != PA_FORM_STREAMS) return pa_fail(PA_ERR_INVALID, "form %d unknown", a->form);
   if (!a->query_start_loc && a->num_tokens != a->batch)
     return pa_fail(PA_ERR_INVALID, "without query_start_loc num_tokens (%d) must be batch (%d)", a->num_tokens, a->batch);
   const int64_t elem = (a->kv_dtype == PA_KV_FP16 || a->kv_dtype == PA_KV_BF16) ? 2 : 1;
@@ -794,7 +1141,7 @@ int build(const pa_prefill_args *a, int maps, PParams *out) {
   const int group = a->num_q_heads / a->num_kv_heads;
   const int units = a->num_kv_heads / maps;
   if ((int64_t)a->num_tokens * a->num_q_heads >= 2 * gib) return pa_fail(PA_ERR_UNSUPPORTED, "num_tokens * num_q_heads must be below 2^31");
-  const int row_tile = kRowsPerWave * kWaves / maps;
+  const int row_tile = a->form == PA_FORM_STREAMS ? kRowsPerWave / maps : kRowsPerWave * kWaves / maps;
   const int seq_tiles = (group + row_tile - 1) / row_tile;
   const int64_t tiles = a->query_start_loc ? (int64_t)a->num_tokens * group / row_tile + a->batch
                                            : (int64_t)a->batch * seq_tiles;
@@ -823,6 +1170,7 @@ int build(const pa_prefill_args *a, int maps, PParams *out) {
   p.max_tokens = a->max_blocks * bs;
   p.log2_page = __builtin_ctz((unsigned)bs);
   p.num_splits = a->num_splits;
+  p.max_seq_len = std::min(a->max_seq_len, p.max_tokens);
   p.tiles = (int32_t)tiles;
   p.sqt = (int32_t)a->stride_qt;
   p.sqh = (int32_t)a->stride_qh;
@@ -849,31 +1197,37 @@ int build(const pa_prefill_args *a, int maps, PParams *out) {
 }
 
 template <int KV, int SC, int D, int MAPS>
-hipError_t launch(const PParams &p, hipStream_t st) {
-  using G = PGeo<KV, D, MAPS>;
-  const uint32_t grid = (uint32_t)(p.tiles * p.units * p.num_splits);
-  hipLaunchKernelGGL((paged_prefill_kernel<KV, SC, D, MAPS>), dim3(grid), dim3(64 * kWaves), 0, st, p);
+hipError_t launch(const PParams &p, bool streams, hipStream_t st) {
+  constexpr int W = D * MAPS;
+  const dim3 grid((uint32_t)(p.tiles * p.units * p.num_splits)), threads(64 * kWaves);
+  if (streams)
+    hipLaunchKernelGGL((paged_stream_kernel<KV, SC, D, MAPS>), grid, threads, 0, st, p);
+  else
+    hipLaunchKernelGGL((paged_prefill_kernel<KV, SC, D, MAPS>), grid, threads, 0, st, p);
   if (p.num_splits > 1) {
-    const uint32_t rows = (uint32_t)p.num_tokens * (uint32_t)(p.num_q_heads / MAPS);
-    hipLaunchKernelGGL((prefill_merge_kernel<G::W, MAPS, G::BN>), dim3((rows + 3) / 4), dim3(256), 0, st, p);
+    const dim3 rows(((uint32_t)p.num_tokens * (uint32_t)(p.num_q_heads / MAPS) + 3) / 4);
+    if (streams)
+      hipLaunchKernelGGL((prefill_merge_kernel<W, MAPS, SGeo<KV, D, MAPS>::kRowTile>), rows, dim3(256), 0, st, p);
+    else
+      hipLaunchKernelGGL((prefill_merge_kernel<W, MAPS, PGeo<KV, D, MAPS>::kRowTile>), rows, dim3(256), 0, st, p);
   }
   return hipGetLastError();
 }
 
 template <int KV, int SC>
-hipError_t launch_kv(const PParams &p, int d, int maps, hipStream_t st) {
+hipError_t launch_kv(const PParams &p, int d, int maps, bool streams, hipStream_t st) {
   if (maps == 1) {
     switch (d) {
-      case 32: return launch<KV, SC, 32, 1>(p, st);
-      case 64: return launch<KV, SC, 64, 1>(p, st);
-      case 128: return launch<KV, SC, 128, 1>(p, st);
-      default: return launch<KV, SC, 256, 1>(p, st);
+      case 32: return launch<KV, SC, 32, 1>(p, streams, st);
+      case 64: return launch<KV, SC, 64, 1>(p, streams, st);
+      case 128: return launch<KV, SC, 128, 1>(p, streams, st);
+      default: return launch<KV, SC, 256, 1>(p, streams, st);
     }
   }
   switch (d) {
-    case 32: return launch<KV, SC, 32, 2>(p, st);
-    case 64: return launch<KV, SC, 64, 2>(p, st);
-    default: return launch<KV, SC, 128, 2>(p, st);
+    case 32: return launch<KV, SC, 32, 2>(p, streams, st);
+    case 64: return launch<KV, SC, 64, 2>(p, streams, st);
+    default: return launch<KV, SC, 128, 2>(p, streams, st);
   }
 }
 
@@ -884,12 +1238,13 @@ int attend(const pa_prefill_args *a, int maps, void *stream) {
   if (p.tiles == 0 || p.num_tokens == 0) return pa_ok();
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int d = a->head_dim;
+  const bool streams = a->form == PA_FORM_STREAMS;
   hipError_t e;
-  if (a->kv_dtype == PA_KV_FP16) e = launch_kv<PA_KV_FP16, PA_SCALE_NONE>(p, d, maps, st);
-  else if (a->kv_dtype == PA_KV_BF16) e = launch_kv<PA_KV_BF16, PA_SCALE_NONE>(p, d, maps, st);
-  else if (a->kv_dtype == PA_KV_FP8_E5M2) e = launch_kv<PA_KV_FP8_E5M2, PA_SCALE_NONE>(p, d, maps, st);
-  else if (a->scale_dtype == PA_SCALE_FP32) e = launch_kv<PA_KV_INT8, PA_SCALE_FP32>(p, d, maps, st);
-  else e = launch_kv<PA_KV_INT8, PA_SCALE_FP16>(p, d, maps, st);
+  if (a->kv_dtype == PA_KV_FP16) e = launch_kv<PA_KV_FP16, PA_SCALE_NONE>(p, d, maps, streams, st);
+  else if (a->kv_dtype == PA_KV_BF16) e = launch_kv<PA_KV_BF16, PA_SCALE_NONE>(p, d, maps, streams, st);
+  else if (a->kv_dtype == PA_KV_FP8_E5M2) e = launch_kv<PA_KV_FP8_E5M2, PA_SCALE_NONE>(p, d, maps, streams, st);
+  else if (a->scale_dtype == PA_SCALE_FP32) e = launch_kv<PA_KV_INT8, PA_SCALE_FP32>(p, d, maps, streams, st);
+  else e = launch_kv<PA_KV_INT8, PA_SCALE_FP16>(p, d, maps, streams, st);
   if (e != hipSuccess) return pa_fail(PA_ERR_HIP, "launch failed: %s", hipGetErrorString(e));
   return pa_ok();
 }

@@ -31,6 +31,9 @@ PA_SCALE_FP32 = 2
 PA_IO_FP16 = 0
 PA_IO_BF16 = 1
 
+PA_FORM_TILES = 0
+PA_FORM_STREAMS = 1
+
 PA_MAX_SPLITS = 4096
 PA_MAX_FLAT_SPLITS = 65536
 PA_MAX_FLAT_SEQ_COST = 64
@@ -186,6 +189,8 @@ class PaPrefillArgs(ctypes.Structure):
         ("num_blocks", _i32),
         ("max_blocks", _i32),
         ("num_splits", _i32),
+        ("max_seq_len", _i32),
+        ("form", _i32),
         ("stride_qt", _i64),
         ("stride_qh", _i64),
         ("stride_kn", _i64),

@@ -17,20 +17,26 @@ from . import _abi
 from .cache import PagedKVCache
 from .hip_decode import _IO_CODE, _KV_CODE, _SCALE_CODE, _STORE_DTYPE, _cu_count, _launch
 
-# Tokens of a kernel tile (csrc/paged_prefill.hip) and rows of a workgroup, by the
-# width of a cache row (a pair of heads for the differential forms).
-ROWS_PER_WORKGROUP = 128
+# Rows of a workgroup (a row is a new token and a head of its kv head's group; in the
+# differential forms, which hold both maps of each, half as many) in the form for
+# many rows and in the one for few, and the average rows a (sequence, kv head) up
+# to which the latter is taken (csrc/paged_prefill.hip).
+TILE_ROWS = 128
+STREAM_ROWS = 32
 # Workgroups that a CU holds at once, and the fewest tokens worth a split.
 WORKGROUPS_PER_CU = 2
 MIN_SPLIT_TOKENS = 256
 
 
-def _plan_splits(row_tiles: int, units: int, longest: int, cus: int) -> int:
-    """How many chunks each row tile's tokens are cut into: enough workgroups
-    for the chip, none below MIN_SPLIT_TOKENS tokens."""
-    work = max(1, row_tiles * units)
+def _plan(rows: int, batch: int, units: int, longest: int, cus: int, maps: int) -> tuple[int, int]:
+    """(form, num_splits) from shapes alone: `rows` (token, head) rows in all for
+    each of `units` kv heads (pairs of them in the differential forms)."""
+    few = rows * maps <= STREAM_ROWS * batch
+    tile = (STREAM_ROWS if few else TILE_ROWS) // maps
+    work = max(1, max(batch, rows // tile) * units)
     want = WORKGROUPS_PER_CU * cus // work
-    return max(1, min(want, -(-longest // MIN_SPLIT_TOKENS), _abi.PA_MAX_SPLITS))
+    splits = max(1, min(want, -(-longest // MIN_SPLIT_TOKENS), _abi.PA_MAX_SPLITS))
+    return (_abi.PA_FORM_STREAMS if few else _abi.PA_FORM_TILES), splits
 
 
 def _attend(fn_name, maps, q, cache, start, out, sm_scale, num_splits, max_seq_len, lam=None, norm_weight=None,
@@ -102,13 +108,10 @@ def _attend(fn_name, maps, q, cache, start, out, sm_scale, num_splits, max_seq_l
             raise ValueError(f"norm_weight must be contiguous float32 [{2 * d}]")
     if n == 0 or b == 0:
         return out
-    group = hq // hkv
-    if num_splits is None:
-        longest = blocks * cache.block_size if max_seq_len is None else min(int(max_seq_len), blocks * cache.block_size)
-        rows = ROWS_PER_WORKGROUP // maps
-        tiles = b * -(-group // rows) if start is None else max(b, n * group // rows + b // 2)
-        num_splits = _plan_splits(tiles, hkv // maps, longest, _cu_count(q.device))
-    num_splits = int(num_splits)
+    capacity = blocks * cache.block_size
+    longest = capacity if max_seq_len is None else max(0, min(int(max_seq_len), capacity))
+    form, planned = _plan(n * (hq // hkv), b, hkv // maps, longest, _cu_count(q.device), maps)
+    num_splits = planned if num_splits is None else int(num_splits)
     po = pl = None
     if num_splits > 1:
         part = torch.empty((num_splits * n * hq * (maps * d + 1),), dtype=torch.float32, device=q.device)
@@ -119,6 +122,7 @@ def _attend(fn_name, maps, q, cache, start, out, sm_scale, num_splits, max_seq_l
         None if start is None else start.data_ptr(), None if lam is None else lam.data_ptr(),
         None if norm_weight is None else norm_weight.data_ptr(),
         b, n, hq, hkv, d, cache.block_size, k.shape[0], blocks, num_splits,
+        0 if max_seq_len is None else longest, form,
         qst[0], qst[1], kst[0], kst[1], kst[2], sst[0], sst[1], ost[0], ost[1],
         bt.stride(0) if b > 1 else blocks, lam_stride,
         _KV_CODE[kv_dtype], scale_code, _IO_CODE[q.dtype], d ** -0.5 if sm_scale is None else float(sm_scale),
@@ -147,9 +151,12 @@ def paged_prefill_hip(
     row i of n_b sees tokens 0 .. T_b - n_b + i. A row that sees none is zeros.
     Rows of no sequence (padding behind the last) are left as they are in `out`.
 
-    `num_splits` cuts each row tile's tokens into that many chunks, joined by a
-    second kernel; None plans it from the shapes alone, with no device sync, by
-    `max_seq_len` (a host int; None: what the block table can hold).
+    `num_splits` cuts each row tile's tokens into at most that many chunks, joined
+    by a second kernel; None plans it from the shapes alone, with no device sync.
+    `max_seq_len` (a host int; None: what the block table can hold) is what it
+    plans by, and, if given, sizes every chunk as of a sequence that long, so a
+    ragged batch's short sequences are cut less. Results do not depend on it
+    beyond rounding, and longer sequences are attended whole.
     """
     return _attend("pa_prefill", 1, q, cache, query_start_loc, out, sm_scale, num_splits, max_seq_len)
 

@@ -8,9 +8,20 @@ import pytest
 import torch
 
 import prompt_oracle as po
-from pagedattn import LLAMA3_8B, MHA_DEBUG, QWEN25_05B, ModelShape, allocate, paged_decode_hip, paged_prefill_hip
+from pagedattn import (LLAMA3_8B, MHA_DEBUG, QWEN25_05B, ModelShape, _abi, allocate, paged_decode_hip,
+                       paged_prefill_hip, prefill)
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, params=["planned", "tiles", "streams"])
+def form(request, monkeypatch):
+    """Every test as the plan has it, and in the form for many rows and the one for few."""
+    if request.param != "planned":
+        plan = prefill._plan
+        code = {"tiles": _abi.PA_FORM_TILES, "streams": _abi.PA_FORM_STREAMS}[request.param]
+        monkeypatch.setattr(prefill, "_plan", lambda *a: (code, plan(*a)[1]))
+    return request.param
 
 WIDE = ModelShape(4, 1, 256, "wide")
 THIN = ModelShape(6, 2, 32, "thin")
@@ -110,11 +121,13 @@ def test_rows_of_no_sequence_are_left():
 
 
 @pytest.mark.parametrize("splits", [1, 2, 3, 7, 40, None])
+@pytest.mark.parametrize("longest", [None, 500, 1500, 5000])
 @pytest.mark.parametrize("shape", [LLAMA3_8B, QWEN25_05B, WIDE], ids=lambda s: s.name)
-def test_splits(shape, splits):
-    """Few rows over long sequences, more splits than tiles among them."""
+def test_splits(shape, splits, longest):
+    """Few rows over long sequences, more splits than tiles among them; the longest length given or
+    not, right or wrong."""
     q, c, start = case(shape, [2, 5, 1], [1500, 3, 64], "int8", torch.float32, seed=7)
-    check(q, c, start, num_splits=splits)
+    check(q, c, start, num_splits=splits, max_seq_len=longest)
 
 
 @pytest.mark.parametrize("batch", [63, 64, 65, 130, 4200])
