@@ -38,52 +38,11 @@
 
 #include <algorithm>
 
-#include "kv_math.h"
-#include "launch_math.h"
 #include "pa_errors.h"
 #include "pagedattn.h"
+#include "prefill_common.h"
 
 namespace {
-
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-
-constexpr int kWaves = 4;
-constexpr int kRowsPerWave = 32;
-constexpr float kRescaleLog2 = 8.0f;
-constexpr int kSplitUnit = 128;  // splits are multiples of this many tokens
-// A lane offset past every buffer (page_rsrc's -1 leaves all others in range):
-// the load returns zeros.
-constexpr uint32_t kOutside = 0xfffffff0u;
-constexpr int kRsrcBytes = (int)kOutside;
-
-struct PParams {
-  const uint8_t *q;
-  const uint8_t *k;
-  const uint8_t *v;
-  const uint8_t *ks;
-  const uint8_t *vs;
-  uint8_t *out;
-  float *part_out;  // [num_splits, num_tokens, num_q_heads, DV]
-  float *part_lse;  // [num_splits, num_tokens, num_q_heads]
-  const int32_t *bt;
-  const int32_t *seq_lens;
-  const int32_t *start;  // [batch + 1] row offsets, or NULL: one row a sequence
-  const float *lam;      // differential: [num_q_heads / 2]
-  const float *norm;     // differential: [DV] or NULL
-  int32_t batch, num_tokens, units, group, num_q_heads;
-  int32_t num_blocks, max_tokens, log2_page, num_splits;
-  int32_t max_seq_len;   // > 0: chunks no shorter than those of a sequence this long
-  int32_t tiles;         // row tiles of the launch
-  int32_t sqt, sqh, sot, soh;  // elements
-  uint32_t skn, skt, skh, ssn, sst;  // bytes
-  int32_t sbtb, slam;    // elements
-  float qk_scale;        // sm_scale * log2(e)
-  float norm_eps, out_scale;
-  int32_t io_bf16;
-  Div by_units, by_splits, by_group, by_seq_tiles, by_heads;
-};
 
 // Compile-time geometry: MAPS maps of head_dim D each, a cache row of W = MAPS *
 // D elements, which is also the width of the value.
@@ -109,77 +68,6 @@ struct PGeo {
   static constexpr int kWavesPerEU = W == 256 ? 1 : 2;
   static_assert(64 / kPPR <= 16 && BN * kPPR % (64 * kWaves) == 0, "a wave's load lies in one page");
 };
-
-// x combined with the value of the other half of the wave (lane ^ 32).
-__device__ __forceinline__ float half_max(float x) {
-  const uint32_t u = __float_as_uint(x);
-  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-}
-
-__device__ __forceinline__ float half_sum(float x) {
-  const uint32_t u = __float_as_uint(x);
-  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
-}
-
-// First row of sequence b among the packed rows, kept inside them whatever the
-// device's offsets hold.
-__device__ __forceinline__ int row_start(const PParams &p, int b) {
-  return p.start ? min(max(ro(p.start)[b], 0), p.num_tokens) : b;
-}
-
-// The sequence whose key(start, b) is the last at or below x, for a key that
-// grows with b: 64 probes at a time.
-template <typename KEY>
-__device__ __forceinline__ int find_sequence(const PParams &p, int x, int lane, KEY key) {
-  int lo = 0, n = p.batch;
-  for (;;) {
-    const int step = (n + 63) / 64;
-    const int b = lo + lane * step;
-    bool below = false;
-    if (lane * step < n) below = key(row_start(p, b), b) <= x;
-    const uint64_t m = __builtin_amdgcn_ballot_w64(below);
-    const int count = m == ~0ull ? 64 : __builtin_ctzll(~m);
-    lo += max(count - 1, 0) * step;
-    if (step == 1) return __builtin_amdgcn_readfirstlane(lo);
-    n = min(step, p.batch - lo);
-  }
-}
-
-// A row tile: its sequence, its first row there, and the tokens that its rows see.
-struct RowTile {
-  int b, row0, rows;  // rows: n_b * group (row0 >= rows: no such tile)
-  int token0;         // first packed row of the sequence
-  int first;          // tokens before the sequence's new ones (negative: fewer than n_b in all)
-  int len;            // T_b
-  int hi;             // tokens seen by the last row of the tile
-};
-
-// `index` of the sequence's tiles of ROWS rows.
-template <int ROWS>
-__device__ __forceinline__ RowTile tile_at(const PParams &p, int b, int index) {
-  RowTile t;
-  t.b = b;
-  t.token0 = row_start(p, b);
-  const int n = p.start ? max(row_start(p, b + 1) - t.token0, 0) : 1;
-  t.rows = n * p.group;
-  t.row0 = index * ROWS;
-  t.len = max(0, min(ro(p.seq_lens)[b], p.max_tokens));
-  t.first = t.len - n;
-  const int last = min(n - 1, (int)div_by((uint32_t)(t.row0 + ROWS - 1), p.by_group));
-  t.hi = max(0, t.first + last + 1);
-  return t;
-}
-
-// Tokens of a split of a row tile that sees `hi`, a multiple of UNIT: the tile's own
-// chunk, or that of a tile that sees max_seq_len if it is larger (ragged batches:
-// long sequences take all splits, short ones few).
-template <int UNIT>
-__device__ __forceinline__ int split_tokens(const PParams &p, int hi) {
-  const uint32_t units = ((uint32_t)max(hi, p.max_seq_len) + UNIT - 1) / UNIT;
-  return (int)div_by(units + p.num_splits - 1, p.by_splits) * UNIT;
-}
 
 template <int KV, int SC, int D, int MAPS>
 struct Staged {
@@ -210,23 +98,6 @@ __device__ __forceinline__ int first_row(int wave, int i) {
   return (64 * wave + 64 * kWaves * i) / G::kPPR;
 }
 
-template <int WORDS>
-__device__ __forceinline__ void load_piece(uint32_t (&w)[WORDS], __amdgpu_buffer_rsrc_t r, uint32_t off) {
-  if constexpr (WORDS == 4) {
-    const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
-    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-  } else {
-    const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
-    w[0] = x.x; w[1] = x.y;
-  }
-}
-
-template <int SC>
-__device__ __forceinline__ uint32_t load_scale(__amdgpu_buffer_rsrc_t r, uint32_t off) {
-  if constexpr (SC == PA_SCALE_FP32) return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
-  else return __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
-}
-
 // The pages of the tile at n0 that this wave loads from. Rows past the sequence
 // take the last token's page (and are read as zeros).
 template <int KV, int D, int MAPS>
@@ -255,8 +126,8 @@ __device__ __forceinline__ void load_tile(Staged<KV, SC, D, MAPS> &st, const PPa
     const uint64_t row0 = (uint64_t)blk * p.skn + in_page * p.skt;
     const bool inside = n0 + la.row[i] < len;
     const uint32_t off = inside ? la.off : kOutside;
-    load_piece(st.k[i], page_rsrc(kbase + row0, kRsrcBytes), off);
-    load_piece(st.v[i], page_rsrc(vbase + row0, kRsrcBytes), off);
+    load_piece<0>(st.k[i], page_rsrc(kbase + row0, kRsrcBytes), off);
+    load_piece<0>(st.v[i], page_rsrc(vbase + row0, kRsrcBytes), off);
     if constexpr (KV == PA_KV_INT8) {
       const uint64_t srow0 = (uint64_t)blk * p.ssn + in_page * p.sst;
       const uint32_t soff = inside ? la.soff : kOutside;
@@ -264,52 +135,6 @@ __device__ __forceinline__ void load_tile(Staged<KV, SC, D, MAPS> &st, const PPa
       st.vs[i] = load_scale<SC>(page_rsrc(vsbase + srow0, kRsrcBytes), soff);
     }
   }
-}
-
-// A piece's elements as fp16 words (two elements each).
-template <int KV, int SC, int WORDS>
-__device__ __forceinline__ void to_halves(uint32_t *h, const uint32_t (&w)[WORDS], uint32_t scale_bits) {
-  if constexpr (KV == PA_KV_FP16) {
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i) h[i] = w[i];
-  } else if constexpr (KV == PA_KV_BF16) {
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i) h[i] = bf16x2_to_f16x2(w[i]);
-  } else if constexpr (KV == PA_KV_FP8_E5M2) {
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i) {
-      h[2 * i] = bytes_to_halves<KV>(w[i], w[i], pair_sel<KV>(0, 1));
-      h[2 * i + 1] = bytes_to_halves<KV>(w[i], w[i], pair_sel<KV>(2, 3));
-    }
-  } else if constexpr (SC == PA_SCALE_FP16) {
-    const uint32_t s2 = scale_bits | (scale_bits << 16);
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i) {
-      h[2 * i] = i8pair_fp16_scale(w[i] ^ kInt8Sign, 0, 1, s2);
-      h[2 * i + 1] = i8pair_fp16_scale(w[i] ^ kInt8Sign, 2, 3, s2);
-    }
-  } else {
-    const float s = __uint_as_float(scale_bits) * kInt8Unit, c = s * (-1.0f / 131072.0f);
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i) {
-      const uint32_t x = w[i] ^ kInt8Sign;
-      h[2 * i] = i8pair_fp32_scale(perm(x, x, pair_sel<KV>(0, 1)), s, c, s, c);
-      h[2 * i + 1] = i8pair_fp32_scale(perm(x, x, pair_sel<KV>(2, 3)), s, c, s, c);
-    }
-  }
-}
-
-// Whether a half of the word is an infinity or NaN.
-__device__ __forceinline__ bool has_wild(uint32_t w) {
-  return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
-}
-
-// Infinities and NaN of the word's halves to zeros; whether there was one.
-__device__ __forceinline__ bool tame_word(uint32_t &w) {
-  if (__builtin_expect(!has_wild(w), 1)) return false;
-  if ((w & 0x7c00u) == 0x7c00u) w &= 0xffff0000u;
-  if ((w & 0x7c000000u) == 0x7c000000u) w &= 0xffffu;
-  return true;
 }
 
 // The staged tile into an LDS buffer (K rows, then V rows). With `tame`,
@@ -338,19 +163,6 @@ __device__ __forceinline__ bool store_tile(uint8_t *buf, const Staged<KV, SC, D,
     for (int w = 0; w < kHalves; w += 4) *reinterpret_cast<u32x4 *>(vd + 4 * w) = u32x4{h[w], h[w + 1], h[w + 2], h[w + 3]};
   }
   return wild;
-}
-
-// The V^T operand of tokens 16 kb .. + 15 and value elements 32 db .. + 31: lane
-// (row d = lane & 31, half h) holds tokens 16 kb + 8 (j / 4) + 4 h + j % 4. Every 16
-// lanes read four rows of 16 elements and get a column each.
-template <int VSTRIDE>
-__device__ __forceinline__ f16x8 read_v(const uint8_t *v, int kb, int db, uint32_t lane_off) {
-  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  const uint8_t *a = v + 16 * kb * VSTRIDE + 64 * db + lane_off;
-  const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)a);
-  const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(a + 8 * VSTRIDE));
-  const u32x2 xa = __builtin_bit_cast(u32x2, x), ya = __builtin_bit_cast(u32x2, y);
-  return as_f16x8(xa.x, xa.y, ya.x, ya.y);
 }
 
 template <int D, int W>
@@ -411,7 +223,8 @@ __device__ __forceinline__ void rescale(RowState<D, W> &st, float top) {
   }
 }
 
-// Scores to P, and O^T += V^T P^T.
+// Scores to P, and O^T += V^T P^T, 16 tokens a product: lane (row d = lane & 31, half
+// h) holds tokens 16 kb + 8 (j / 4) + 4 h + j % 4 of V^T, as the scores lie.
 template <int VSTRIDE, int D, int W, int NB>
 __device__ __forceinline__ void accumulate(RowState<D, W> &st, f32x16 (&s)[NB], const uint8_t *v, uint32_t v_lane,
                                            float qk_scale) {
@@ -437,7 +250,7 @@ __device__ __forceinline__ void accumulate(RowState<D, W> &st, f32x16 (&s)[NB], 
     const f16x8 pop = as_f16x8(w[0], w[1], w[2], w[3]);
 #pragma unroll
     for (int d = 0; d < W / 32; ++d)
-      st.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(read_v<VSTRIDE>(v, kb, d, v_lane), pop, st.acc[d], 0, 0, 0);
+      st.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(read_columns(v + 16 * kb * VSTRIDE + 64 * d + v_lane, 8 * VSTRIDE), pop, st.acc[d], 0, 0, 0);
   }
 }
 
@@ -465,51 +278,6 @@ __device__ __forceinline__ void add_wild(RowState<D, W> &st, const uint8_t *v, i
   }
 }
 
-// Four neighbouring elements of a result row.
-__device__ __forceinline__ void store4(uint8_t *dst, float a, float b, float c, float d, bool bf16) {
-  u32x2 w;
-  if (bf16) {
-    w = u32x2{f32_to_bf16_bits(a) | (f32_to_bf16_bits(b) << 16), f32_to_bf16_bits(c) | (f32_to_bf16_bits(d) << 16)};
-  } else {
-    w = u32x2{cvt_pk_f16(a, b), cvt_pk_f16(c, d)};
-  }
-  *reinterpret_cast<u32x2 *>(dst) = w;
-}
-
-// A lane's accumulators (elements 32 d + 2 i + 4 h .. + 3 in acc[d][i .. i + 3], i a
-// multiple of 4) as an output row: times f, and with `normed` times the norm's
-// weight if there is one.
-template <int W>
-__device__ __forceinline__ void store_rows(const PParams &p, const f32x16 *acc, float f, bool normed, int packed,
-                                           int out_head, int h) {
-  uint8_t *dst = p.out + 2 * ((int64_t)packed * p.sot + (int64_t)out_head * p.soh + 4 * h);
-  const float *norm = normed ? p.norm : nullptr;
-#pragma unroll
-  for (int d = 0; d < W / 32; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      f32x4 y = {acc[d][i] * f, acc[d][i + 1] * f, acc[d][i + 2] * f, acc[d][i + 3] * f};
-      if (norm) y *= *reinterpret_cast<const f32x4 *>(norm + 32 * d + 2 * i + 4 * h);
-      store4(dst + 2 * (32 * d + 2 * i), y.x, y.y, y.z, y.w, p.io_bf16);
-    }
-}
-
-// The same as a partial: normalised, and its log2-sum-exp.
-template <int W>
-__device__ __forceinline__ void store_partial(const PParams &p, const f32x16 *acc, float m, float l, int split,
-                                              int packed, int head, int h) {
-  const int64_t at = ((int64_t)split * p.num_tokens + packed) * p.num_q_heads + head;
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  float *dst = p.part_out + at * W + 4 * h;
-#pragma unroll
-  for (int d = 0; d < W / 32; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; i += 4)
-      *reinterpret_cast<f32x4 *>(dst + 32 * d + 2 * i) =
-          f32x4{acc[d][i] * inv, acc[d][i + 1] * inv, acc[d][i + 2] * inv, acc[d][i + 3] * inv};
-  if (h == 0) p.part_lse[at] = l == 0.f ? -INFINITY : m + __log2f(l);
-}
-
 template <int KV, int SC, int D, int MAPS>
 __global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(PGeo<KV, D, MAPS>::kWavesPerEU)))
 paged_prefill_kernel(const PParams p) {
@@ -524,14 +292,16 @@ paged_prefill_kernel(const PParams p) {
   const int map = MAPS == 2 ? wave & 1 : 0;
   const int wave_row = kRowsPerWave * (wave / MAPS);
 
-  // blockIdx = (tile * num_splits + split) * units + unit: the units (kv heads)
-  // of the same tokens run together, and with 8 of them each XCD keeps one
-  // head's K/V in its L2. Tiles go from the last, which see the most tokens.
+  // blockIdx = (split * tiles + tile) * units + unit: the units (kv heads) of the
+  // same tokens run together, and with 8 of them each XCD keeps one head's K/V in
+  // its L2. Tiles go from the last, which see the most tokens. Splits are
+  // outermost: the later ones hold tokens of the longest sequences only, and a CU
+  // that the round-robin gave always the same split would have all or no work
+  // (24 sequences of 500-8,000 tokens in 4 splits 85.7 us, in 3 65.1).
   const uint32_t x1 = div_by(blockIdx.x, p.by_units);
   const int unit = blockIdx.x - x1 * p.units;
-  const uint32_t x2 = div_by(x1, p.by_splits);
-  const int split = x1 - x2 * p.num_splits;
-  const int tile = p.tiles - 1 - (int)x2;
+  const int split = div_by(x1, p.by_tiles);
+  const int tile = p.tiles - 1 - (int)(x1 - (uint32_t)split * p.tiles);
 
   int b, index;
   if (p.start) {
@@ -650,14 +420,15 @@ paged_prefill_kernel(const PParams p) {
   }
 
   const float l = half_sum(st.l);
+  auto element = [&](int e) { return st.acc[e / 16][e % 16]; };
   if (!direct) {
-    if (live) store_partial<W>(p, st.acc, st.m, l, split, rt.token0 + token, head, h);
+    if (live) store_partial<W, 32>(p, element, st.m, l, split, rt.token0 + token, head, lane);
     return;
   }
   // (a row that sees nothing is zeros; one whose visible scores are all -inf is 0 / 0)
   float inv = lim < 0 ? 0.f : 1.0f / l;
   if constexpr (MAPS == 1) {
-    if (live) store_rows<W>(p, st.acc, inv, false, rt.token0 + token, head, h);
+    if (live) store_rows<W, 32>(p, element, inv, false, rt.token0 + token, head, lane);
   } else {
     float *other = reinterpret_cast<float *>(sm) + (wave / 2) * (W / 2) * 64;
     __syncthreads();  // every wave is done with the tiles
@@ -681,390 +452,8 @@ paged_prefill_kernel(const PParams p) {
     sq = half_sum(sq);
     if (!live) return;
     const float f = p.norm ? __builtin_amdgcn_rsqf(sq * (1.0f / W) + p.norm_eps) * p.out_scale : 1.0f;
-    store_rows<W>(p, st.acc, f, true, rt.token0 + token, head / 2, h);
+    store_rows<W, 32>(p, element, f, true, rt.token0 + token, head / 2, lane);
   }
-}
-
-// ----------------------------------------------------------------------------
-// Few rows: 32 columns of S^T hold all rows of a (sequence, kv head), or of 16 of
-// its (token, head) pairs with both maps (columns 0-15 and 16-31). Then the four
-// waves of a workgroup share rows, not tokens: wave w takes the 32-token tiles w,
-// w + 4, ... of the workgroup's range, through LDS of its own, with no barrier
-// until the end, where the four are joined as splits are. What bounds it is the
-// stream of K and V: a wave's next tile is in flight while it computes one.
-//
-// The maps of a differential row differ in the half of the K row they meet: each
-// half's products are summed on their own, with q zero in the other map's
-// columns, and a lane keeps its column's sum (what the other half holds,
-// infinities too, stays out of it).
-// ----------------------------------------------------------------------------
-
-template <int KV, int D, int MAPS>
-struct SGeo {
-  static constexpr int W = D * MAPS;
-  static constexpr int kElem = (KV == PA_KV_FP16 || KV == PA_KV_BF16) ? 2 : 1;
-  static constexpr int kPieceBytes = W * kElem >= 64 ? 16 : 8;
-  static constexpr int kPieceElems = kPieceBytes / kElem;
-  static constexpr int kPieceWords = kPieceBytes / 4;
-  static constexpr int kPPR = W / kPieceElems;     // 4 .. 32
-  static constexpr int kIter = 32 * kPPR / 64;     // loads of K (and of V) a tile
-  static constexpr int kKStride = W * 2 + 16;
-  static constexpr int kVStride = W == 32 ? 64 : W * 2 + 64;
-  static constexpr int kSlot = 32 * (kKStride + kVStride);  // LDS of a wave
-  static constexpr int kKSteps = W / 16;
-  static constexpr int kDB = W / 32;
-  static constexpr int kRowTile = 32 / MAPS;
-  static constexpr int kWavesPerEU = W == 256 ? 1 : 2;
-  // Rows of 512 bytes: K and V take turns in the same registers (both at once, with
-  // accumulators and q, do not fit 512); a wave then has 16 KB in flight as others do.
-  static constexpr bool kTurns = W * kElem > 256;
-};
-
-// K or V of a tile on its way to LDS.
-template <int KV, int D, int MAPS>
-struct StreamHalf {
-  using G = SGeo<KV, D, MAPS>;
-  uint32_t w[G::kIter][G::kPieceWords];
-  uint32_t scale[KV == PA_KV_INT8 ? G::kIter : 1];
-};
-
-template <int KV, int SC, int D, int MAPS>
-__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(SGeo<KV, D, MAPS>::kWavesPerEU)))
-paged_stream_kernel(const PParams p) {
-  using G = SGeo<KV, D, MAPS>;
-  constexpr int W = G::W;
-  constexpr int kAccBytes = (kWaves - 1) * (W / 2) * 64 * 4;
-  constexpr int kBytes = kWaves * G::kSlot > kAccBytes ? kWaves * G::kSlot : kAccBytes;
-  __shared__ __attribute__((aligned(16))) uint8_t sm[kBytes];
-  __shared__ float sm_m[kWaves][32], sm_l[kWaves][32];
-
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 31, h = lane >> 5;
-  const int map = MAPS == 2 ? col >> 4 : 0;
-
-  // blockIdx = (tile * num_splits + split) * units + unit
-  const uint32_t x1 = div_by(blockIdx.x, p.by_units);
-  const int unit = blockIdx.x - x1 * p.units;
-  const uint32_t x2 = div_by(x1, p.by_splits);
-  const int split = x1 - x2 * p.num_splits;
-  const int tile = (int)x2;
-  int b, index;
-  if (p.start) {
-    auto key = [&](int start, int seq) { return (int)((uint32_t)(start * p.group) / G::kRowTile) + seq; };
-    b = find_sequence(p, tile, lane, key);
-    index = tile - key(row_start(p, b), b);
-    if (index < 0) return;
-  } else {
-    b = div_by(tile, p.by_seq_tiles);
-    index = tile - b * p.by_seq_tiles.d;
-  }
-  const RowTile rt = tile_at<G::kRowTile>(p, b, index);
-  if (rt.row0 >= rt.rows) return;
-  int lo = 0, hi = rt.hi;
-  bool direct = true;
-  if (p.num_splits > 1) {
-    const int chunk = split_tokens<kSplitUnit>(p, rt.hi);
-    if (split > 0 && (int64_t)split * chunk >= rt.hi) return;
-    lo = split * chunk;
-    hi = min(rt.hi, lo + chunk);
-    direct = rt.hi <= chunk;
-  }
-
-  const int row = rt.row0 + (MAPS == 2 ? col & 15 : col);
-  const bool live = row < rt.rows;
-  const int r = min(row, rt.rows - 1);
-  const int token = div_by((uint32_t)r, p.by_group);
-  const int head = MAPS * (unit * p.group + (r - token * p.group)) + map;
-  const int lim = rt.first + token;
-  const int least = rt.first + (int)div_by((uint32_t)rt.row0, p.by_group) + 1;  // tokens that the first row sees
-
-  RowState<W, W> st;
-  st.m = -INFINITY;
-  st.l = 0.f;
-#pragma unroll
-  for (int d = 0; d < G::kDB; ++d) st.acc[d] = f32x16{};
-  {
-    const uint16_t *qrow = reinterpret_cast<const uint16_t *>(p.q) + (int64_t)(rt.token0 + token) * p.sqt +
-                           (int64_t)head * p.sqh + 8 * h;
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      const u32x4 w = *reinterpret_cast<const u32x4 *>(qrow + 16 * ks);
-      const f16x8 x = p.io_bf16 ? bf16x8_to_f16x8(w) : __builtin_bit_cast(f16x8, w);
-      if constexpr (MAPS == 1) {
-        st.q[ks] = x;
-      } else {
-        st.q[ks] = map == 0 ? x : f16x8{};
-        st.q[D / 16 + ks] = map == 1 ? x : f16x8{};
-      }
-    }
-  }
-
-  // this lane's piece of a load: row (of 64 / kPPR), element
-  const int row_in = lane / G::kPPR;
-  const int ecol = lane % G::kPPR * G::kPieceElems;
-  const uint32_t part = (uint32_t)ecol / D;
-  const uint32_t off = row_in * p.skt + part * p.skh + ((uint32_t)ecol - part * D) * G::kElem;
-  const uint32_t soff = row_in * p.sst + part * (SC == PA_SCALE_FP32 ? 4 : 2);
-  const int64_t head_off = (int64_t)unit * MAPS * p.skh;
-  const int64_t scale_off = (int64_t)unit * MAPS * (SC == PA_SCALE_FP32 ? 4 : 2);
-  const ro_i32 *bt_row = ro(p.bt) + (int64_t)rt.b * p.sbtb;
-  uint8_t *slot = sm + wave * G::kSlot;
-
-  // tile at n0 (a multiple of 32: a 16-token half lies in one page)
-  auto pages = [&](int n0, int (&pg)[2]) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) pg[u] = bt_row[(uint32_t)min(n0 + 16 * u, rt.len - 1) >> p.log2_page];
-  };
-  StreamHalf<KV, D, MAPS> first_half, second_half;
-  auto &tk = first_half;
-  auto &tv = G::kTurns ? first_half : second_half;
-  auto load = [&](StreamHalf<KV, D, MAPS> &t, const uint8_t *base, const uint8_t *sbase, int n0, const int (&pg)[2]) {
-#pragma unroll
-    for (int i = 0; i < G::kIter; ++i) {
-      const int r0 = i * (64 / G::kPPR);  // first row of the load
-      const uint32_t blk = (uint32_t)min(max(pg[r0 / 16], 0), p.num_blocks - 1);
-      const uint32_t in_page = (uint32_t)(n0 + r0) & ((1u << p.log2_page) - 1u);
-      const bool inside = n0 + r0 + row_in < rt.len;
-      load_piece(t.w[i], page_rsrc(base + head_off + (uint64_t)blk * p.skn + in_page * p.skt, kRsrcBytes),
-                 inside ? off : kOutside);
-      if constexpr (KV == PA_KV_INT8)
-        t.scale[i] = load_scale<SC>(page_rsrc(sbase + scale_off + (uint64_t)blk * p.ssn + in_page * p.sst, kRsrcBytes),
-                                    inside ? soff : kOutside);
-    }
-  };
-  auto load_k = [&](int n0, const int (&pg)[2]) { load(tk, p.k, p.ks, n0, pg); };
-  auto load_v = [&](int n0, const int (&pg)[2]) { load(tv, p.v, p.vs, n0, pg); };
-  // into the wave's slot; with `tame` as store_tile does for V
-  auto store = [&](const StreamHalf<KV, D, MAPS> &t, uint8_t *dst, int stride, bool tame) {
-    bool wild = false;
-#pragma unroll
-    for (int i = 0; i < G::kIter; ++i) {
-      constexpr int kHalves = G::kPieceElems / 2;
-      uint32_t x[kHalves];
-      to_halves<KV, SC>(x, t.w[i], KV == PA_KV_INT8 ? t.scale[KV == PA_KV_INT8 ? i : 0] : 0);
-      if (tame) {
-#pragma unroll
-        for (int w = 0; w < kHalves; ++w) wild |= tame_word(x[w]);
-      }
-      uint8_t *d = dst + (i * (64 / G::kPPR) + row_in) * stride + ecol * 2;
-#pragma unroll
-      for (int w = 0; w < kHalves; w += 4) *reinterpret_cast<u32x4 *>(d + 4 * w) = u32x4{x[w], x[w + 1], x[w + 2], x[w + 3]};
-    }
-    return wild;
-  };
-  auto store_k = [&] { store(tk, slot, G::kKStride, false); };
-  auto store_v = [&](bool tame) { return store(tv, slot + 32 * G::kKStride, G::kVStride, tame); };
-  auto sync_slot = [] {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  };
-
-  const uint8_t *k_lane = slot + col * G::kKStride + 16 * h;
-  const uint8_t *v_slot = slot + 32 * G::kKStride;
-  const uint32_t v_lane = (4 * h + ((lane & 15) >> 2)) * G::kVStride + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-  const int n_first = lo + 32 * wave;
-  bool wild = false;
-  if (n_first < hi) {
-    int pg[2];
-    pages(n_first, pg);
-    load_k(n_first, pg);
-    if constexpr (G::kTurns) store_k();
-    load_v(n_first, pg);
-    pages(n_first + 32 * kWaves, pg);
-    for (int n0 = n_first; n0 < hi; n0 += 32 * kWaves) {
-      const bool masked = n0 + 32 > least;
-      const int next = n0 + 32 * kWaves;
-      if constexpr (!G::kTurns) {
-        store_k();
-        wild |= store_v(masked);
-      }
-      sync_slot();
-      if (!G::kTurns && next < hi) {
-        load_k(next, pg);
-        load_v(next, pg);
-        pages(next + 32 * kWaves, pg);
-      }
-      f32x16 s[1];
-      if constexpr (MAPS == 1) {
-        scores_of<G::kKSteps, G::kKStride>(s, st.q, k_lane);
-      } else {
-        f32x16 s2[1];
-        scores_of<G::kKSteps / 2, G::kKStride>(s, st.q, k_lane);
-        scores_of<G::kKSteps / 2, G::kKStride>(s2, st.q + G::kKSteps / 2, k_lane + 2 * D);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[0][i] = map == 1 ? s2[0][i] : s[0][i];
-      }
-      if (masked) {
-        asm volatile("");  // a branch
-        mask(s, n0, lim, h);
-      }
-      rescale(st, top_score(s, p.qk_scale));
-      if constexpr (G::kTurns) {
-        wild |= store_v(masked);
-        sync_slot();
-        if (next < hi) load_k(next, pg);
-      }
-      accumulate<G::kVStride>(st, s, v_slot, v_lane, p.qk_scale);
-      sync_slot();
-      if (G::kTurns && next < hi) {
-        store_k();
-        load_v(next, pg);
-        pages(next + 32 * kWaves, pg);
-      }
-    }
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(wild) != 0, 0)) {
-      for (int n0 = n_first; n0 < hi; n0 += 32 * kWaves) {
-        if (n0 + 32 <= least) continue;
-        pages(n0, pg);
-        load_v(n0, pg);
-        store_v(false);
-        sync_slot();
-        add_wild<32, G::kVStride>(st, v_slot, n0, lim, lane);
-        sync_slot();
-      }
-    }
-  }
-
-  // join the waves
-  const float lw = half_sum(st.l);
-  if (h == 0) {
-    sm_m[wave][col] = st.m;
-    sm_l[wave][col] = lw;
-  }
-  __syncthreads();  // (and every wave is done with its slot)
-  float m = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, sm_m[w][col]);
-  float l = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const float mw = sm_m[w][col];
-    // (a wave that saw nothing of the row has a sum of zero)
-    l += mw == -INFINITY ? sm_l[w][col] : sm_l[w][col] * __builtin_amdgcn_exp2f(mw - m);
-  }
-  const float f = st.m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m - m);
-  float *others = reinterpret_cast<float *>(sm);
-  if (wave > 0) {
-#pragma unroll
-    for (int d = 0; d < G::kDB; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) others[((wave - 1) * (W / 2) + 16 * d + i) * 64 + lane] = st.acc[d][i] * f;
-  }
-  __syncthreads();
-  if (wave > 0) return;
-#pragma unroll
-  for (int d = 0; d < G::kDB; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float a = st.acc[d][i] * f;
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) a += others[((w - 1) * (W / 2) + 16 * d + i) * 64 + lane];
-      st.acc[d][i] = a;
-    }
-  if (!direct) {
-    if (live) store_partial<W>(p, st.acc, m, l, split, rt.token0 + token, head, h);
-    return;
-  }
-  float inv = lim < 0 ? 0.f : 1.0f / l;
-  if constexpr (MAPS == 1) {
-    if (live) store_rows<W>(p, st.acc, inv, false, rt.token0 + token, head, h);
-  } else {
-    // columns c and c + 16 (lanes apart by 16) hold the maps of a row
-    if (map == 1) inv *= p.lam[(int64_t)(head / 2) * p.slam];
-    float sq = 0.f;
-#pragma unroll
-    for (int d = 0; d < G::kDB; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint32_t x = __float_as_uint(st.acc[d][i] * inv);
-        const auto two = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-        const float y = __uint_as_float(two[0]) - __uint_as_float(two[1]);
-        st.acc[d][i] = y;
-        sq += y * y;
-      }
-    sq = half_sum(sq);
-    if (live && map == 0) {
-      const float scale = p.norm ? __builtin_amdgcn_rsqf(sq * (1.0f / W) + p.norm_eps) * p.out_scale : 1.0f;
-      store_rows<W>(p, st.acc, scale, true, rt.token0 + token, head / 2, h);
-    }
-  }
-}
-
-// Joins the partials of a split launch: one wave an output row, W / 64 elements a
-// lane (W = 32: the upper half of the wave idles). Row tiles of one split are done;
-// empty splits were not written and are not read.
-template <int W, int MAPS, int ROWS>
-__global__ void __launch_bounds__(256) prefill_merge_kernel(const PParams p) {
-  constexpr int E = W >= 64 ? W / 64 : 1;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t out_heads = p.num_q_heads / MAPS;
-  const uint32_t x = blockIdx.x * 4u + wave;  // row * out_heads + head
-  if (x >= (uint32_t)p.num_tokens * out_heads) return;
-  const int packed = div_by(x, p.by_heads);
-  const int out_head = x - packed * out_heads;
-  int b = packed;
-  if (p.start) {
-    b = find_sequence(p, packed, lane, [](int start, int) { return start; });
-    const int s0 = row_start(p, b), s1 = row_start(p, b + 1);
-    if (packed < s0 || packed >= s1) return;  // a row of no sequence
-  }
-  const int token = packed - row_start(p, b);
-  const int in_group = out_head % p.group;
-  const RowTile rt = tile_at<ROWS>(p, b, (token * p.group + in_group) / ROWS);
-  const int chunk = split_tokens<kSplitUnit>(p, rt.hi);
-  if (rt.hi <= chunk) return;  // written by its one workgroup
-  const int n = (rt.hi - 1) / chunk + 1;
-  const bool sees = rt.first + token >= 0;
-
-  float y[E] = {};
-  const int d0 = E * lane;
-  const bool mine = d0 < W;
-#pragma unroll
-  for (int map = 0; map < MAPS; ++map) {
-    const int64_t at = (int64_t)packed * p.num_q_heads + MAPS * out_head + map;
-    const int64_t step = (int64_t)p.num_tokens * p.num_q_heads;
-    float m = -INFINITY, sum = 0.f, acc[E] = {};
-    for (int s = 0; s < n; ++s) {
-      const float lse = p.part_lse[at + s * step];
-      float o[E] = {};
-      if (mine) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = p.part_out[(at + s * step) * W + d0 + e];
-      }
-      if (lse == -INFINITY) continue;
-      const float m_new = lse > m ? lse : m;
-      const float old = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
-      const float w = __builtin_amdgcn_exp2f(lse - m_new);
-      sum = sum * old + w;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = acc[e] * old + w * o[e];
-      m = m_new;
-    }
-    const float inv = sees ? 1.0f / sum : 0.f;
-    const float f = map == 1 ? -inv * p.lam[(int64_t)out_head * p.slam] : inv;
-#pragma unroll
-    for (int e = 0; e < E; ++e) y[e] += acc[e] * f;
-  }
-  if constexpr (MAPS == 2) {
-    if (p.norm) {
-      float sq = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) sq += y[e] * y[e];
-#pragma unroll
-      for (int o = 1; o < 64; o *= 2) sq += __shfl_xor(sq, o);
-      const float f = __builtin_amdgcn_rsqf(sq * (1.0f / W) + p.norm_eps) * p.out_scale;
-#pragma unroll
-      for (int e = 0; e < E; ++e) y[e] *= f * (mine ? p.norm[d0 + e] : 0.f);
-    }
-  }
-  if (!mine) return;
-  uint16_t *dst = reinterpret_cast<uint16_t *>(p.out) + (int64_t)packed * p.sot + (int64_t)out_head * p.soh + d0;
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    dst[e] = p.io_bf16 ? (uint16_t)f32_to_bf16_bits(y[e]) : __builtin_bit_cast(uint16_t, (_Float16)y[e]);
 }
 
 bool fits_i32(int64_t x) { return x >= 0 && x < (int64_t(1) << 31); }
@@ -1094,7 +483,7 @@ int build(const pa_prefill_args *a, int maps, PParams *out) {
   if (a->num_splits > 1 && (!a->part_out || !a->part_lse))
     return pa_fail(PA_ERR_INVALID, "num_splits %d needs part_out and part_lse", a->num_splits);
   if (a->max_seq_len < 0) return pa_fail(PA_ERR_INVALID, "max_seq_len %d < 0", a->max_seq_len);
-  if (a->form != PA_FORM_TILES && a->form != PA_FORM_STREAMS) return pa_fail(PA_ERR_INVALID, "form %d unknown", a->form);
+  if (a->form < PA_FORM_TILES || a->form > PA_FORM_STREAMS16) return pa_fail(PA_ERR_INVALID, "form %d unknown", a->form);
   if (!a->query_start_loc && a->num_tokens != a->batch)
     return pa_fail(PA_ERR_INVALID, "without query_start_loc num_tokens (%d) must be batch (%d)", a->num_tokens, a->batch);
   const int64_t elem = (a->kv_dtype == PA_KV_FP16 || a->kv_dtype == PA_KV_BF16) ? 2 : 1;
@@ -1141,7 +530,8 @@ int build(const pa_prefill_args *a, int maps, PParams *out) {
   const int group = a->num_q_heads / a->num_kv_heads;
   const int units = a->num_kv_heads / maps;
   if ((int64_t)a->num_tokens * a->num_q_heads >= 2 * gib) return pa_fail(PA_ERR_UNSUPPORTED, "num_tokens * num_q_heads must be below 2^31");
-  const int row_tile = a->form == PA_FORM_STREAMS ? kRowsPerWave / maps : kRowsPerWave * kWaves / maps;
+  const int columns = a->form == PA_FORM_TILES ? kRowsPerWave * kWaves : a->form == PA_FORM_STREAMS ? 32 : 16;
+  const int row_tile = columns / maps;
   const int seq_tiles = (group + row_tile - 1) / row_tile;
   const int64_t tiles = a->query_start_loc ? (int64_t)a->num_tokens * group / row_tile + a->batch
                                            : (int64_t)a->batch * seq_tiles;
@@ -1189,6 +579,7 @@ int build(const pa_prefill_args *a, int maps, PParams *out) {
   p.io_bf16 = a->io_dtype == PA_IO_BF16;
   p.by_units = make_div(units);
   p.by_splits = make_div(a->num_splits);
+  p.by_tiles = make_div((uint32_t)std::max<int64_t>(tiles, 1));
   p.by_group = make_div(group);
   p.by_seq_tiles = make_div(seq_tiles);
   p.by_heads = make_div(a->num_q_heads / maps);
@@ -1197,37 +588,28 @@ int build(const pa_prefill_args *a, int maps, PParams *out) {
 }
 
 template <int KV, int SC, int D, int MAPS>
-hipError_t launch(const PParams &p, bool streams, hipStream_t st) {
-  constexpr int W = D * MAPS;
-  const dim3 grid((uint32_t)(p.tiles * p.units * p.num_splits)), threads(64 * kWaves);
-  if (streams)
-    hipLaunchKernelGGL((paged_stream_kernel<KV, SC, D, MAPS>), grid, threads, 0, st, p);
-  else
-    hipLaunchKernelGGL((paged_prefill_kernel<KV, SC, D, MAPS>), grid, threads, 0, st, p);
-  if (p.num_splits > 1) {
-    const dim3 rows(((uint32_t)p.num_tokens * (uint32_t)(p.num_q_heads / MAPS) + 3) / 4);
-    if (streams)
-      hipLaunchKernelGGL((prefill_merge_kernel<W, MAPS, SGeo<KV, D, MAPS>::kRowTile>), rows, dim3(256), 0, st, p);
-    else
-      hipLaunchKernelGGL((prefill_merge_kernel<W, MAPS, PGeo<KV, D, MAPS>::kRowTile>), rows, dim3(256), 0, st, p);
-  }
+hipError_t launch(const PParams &p, hipStream_t st) {
+  using G = PGeo<KV, D, MAPS>;
+  hipLaunchKernelGGL((paged_prefill_kernel<KV, SC, D, MAPS>), dim3((uint32_t)(p.tiles * p.units * p.num_splits)),
+                     dim3(64 * kWaves), 0, st, p);
+  if (p.num_splits > 1) launch_merge<G::W, MAPS, G::kRowTile>(p, st);
   return hipGetLastError();
 }
 
 template <int KV, int SC>
-hipError_t launch_kv(const PParams &p, int d, int maps, bool streams, hipStream_t st) {
+hipError_t launch_kv(const PParams &p, int d, int maps, hipStream_t st) {
   if (maps == 1) {
     switch (d) {
-      case 32: return launch<KV, SC, 32, 1>(p, streams, st);
-      case 64: return launch<KV, SC, 64, 1>(p, streams, st);
-      case 128: return launch<KV, SC, 128, 1>(p, streams, st);
-      default: return launch<KV, SC, 256, 1>(p, streams, st);
+      case 32: return launch<KV, SC, 32, 1>(p, st);
+      case 64: return launch<KV, SC, 64, 1>(p, st);
+      case 128: return launch<KV, SC, 128, 1>(p, st);
+      default: return launch<KV, SC, 256, 1>(p, st);
     }
   }
   switch (d) {
-    case 32: return launch<KV, SC, 32, 2>(p, streams, st);
-    case 64: return launch<KV, SC, 64, 2>(p, streams, st);
-    default: return launch<KV, SC, 128, 2>(p, streams, st);
+    case 32: return launch<KV, SC, 32, 2>(p, st);
+    case 64: return launch<KV, SC, 64, 2>(p, st);
+    default: return launch<KV, SC, 128, 2>(p, st);
   }
 }
 
@@ -1238,13 +620,13 @@ int attend(const pa_prefill_args *a, int maps, void *stream) {
   if (p.tiles == 0 || p.num_tokens == 0) return pa_ok();
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int d = a->head_dim;
-  const bool streams = a->form == PA_FORM_STREAMS;
   hipError_t e;
-  if (a->kv_dtype == PA_KV_FP16) e = launch_kv<PA_KV_FP16, PA_SCALE_NONE>(p, d, maps, streams, st);
-  else if (a->kv_dtype == PA_KV_BF16) e = launch_kv<PA_KV_BF16, PA_SCALE_NONE>(p, d, maps, streams, st);
-  else if (a->kv_dtype == PA_KV_FP8_E5M2) e = launch_kv<PA_KV_FP8_E5M2, PA_SCALE_NONE>(p, d, maps, streams, st);
-  else if (a->scale_dtype == PA_SCALE_FP32) e = launch_kv<PA_KV_INT8, PA_SCALE_FP32>(p, d, maps, streams, st);
-  else e = launch_kv<PA_KV_INT8, PA_SCALE_FP16>(p, d, maps, streams, st);
+  if (a->form != PA_FORM_TILES) e = launch_streams(p, a, maps, st);
+  else if (a->kv_dtype == PA_KV_FP16) e = launch_kv<PA_KV_FP16, PA_SCALE_NONE>(p, d, maps, st);
+  else if (a->kv_dtype == PA_KV_BF16) e = launch_kv<PA_KV_BF16, PA_SCALE_NONE>(p, d, maps, st);
+  else if (a->kv_dtype == PA_KV_FP8_E5M2) e = launch_kv<PA_KV_FP8_E5M2, PA_SCALE_NONE>(p, d, maps, st);
+  else if (a->scale_dtype == PA_SCALE_FP32) e = launch_kv<PA_KV_INT8, PA_SCALE_FP32>(p, d, maps, st);
+  else e = launch_kv<PA_KV_INT8, PA_SCALE_FP16>(p, d, maps, st);
   if (e != hipSuccess) return pa_fail(PA_ERR_HIP, "launch failed: %s", hipGetErrorString(e));
   return pa_ok();
 }

@@ -33,6 +33,7 @@ PA_IO_BF16 = 1
 
 PA_FORM_TILES = 0
 PA_FORM_STREAMS = 1
+PA_FORM_STREAMS16 = 2
 
 PA_MAX_SPLITS = 4096
 PA_MAX_FLAT_SPLITS = 65536

@@ -17,26 +17,35 @@ from . import _abi
 from .cache import PagedKVCache
 from .hip_decode import _IO_CODE, _KV_CODE, _SCALE_CODE, _STORE_DTYPE, _cu_count, _launch
 
-# Rows of a workgroup (a row is a new token and a head of its kv head's group; in the
-# differential forms, which hold both maps of each, half as many) in the form for
-# many rows and in the one for few, and the average rows a (sequence, kv head) up
-# to which the latter is taken (csrc/paged_prefill.hip).
-TILE_ROWS = 128
-STREAM_ROWS = 32
-# Workgroups that a CU holds at once, and the fewest tokens worth a split.
-WORKGROUPS_PER_CU = 2
+# Columns of a workgroup's score products, by form (csrc/paged_prefill.hip,
+# csrc/paged_stream.hip): rows, a row being a new token and a head of its kv head's
+# group; the differential forms take two columns a row, one for each map.
+_COLUMNS = {_abi.PA_FORM_TILES: 128, _abi.PA_FORM_STREAMS: 32, _abi.PA_FORM_STREAMS16: 16}
+# Workgroups that a CU holds at once, by form and elements of a cache row.
+_PER_CU = {_abi.PA_FORM_TILES: {256: 1}, _abi.PA_FORM_STREAMS: {256: 1}, _abi.PA_FORM_STREAMS16: {256: 2, 128: 4}}
+# A split is a multiple of this many tokens; fewer than MIN_SPLIT_TOKENS are not
+# worth a partial and its share of the merge.
 MIN_SPLIT_TOKENS = 256
+# Launches with less than this share of the chip's workgroups are split.
+SPLIT_BELOW = 0.85
 
 
-def _plan(rows: int, batch: int, units: int, longest: int, cus: int, maps: int) -> tuple[int, int]:
+def _plan(rows: int, batch: int, units: int, longest: int, cus: int, width: int, maps: int) -> tuple[int, int]:
     """(form, num_splits) from shapes alone: `rows` (token, head) rows in all for
-    each of `units` kv heads (pairs of them in the differential forms)."""
-    few = rows * maps <= STREAM_ROWS * batch
-    tile = (STREAM_ROWS if few else TILE_ROWS) // maps
-    work = max(1, max(batch, rows // tile) * units)
-    want = WORKGROUPS_PER_CU * cus // work
-    splits = max(1, min(want, -(-longest // MIN_SPLIT_TOKENS), _abi.PA_MAX_SPLITS))
-    return (_abi.PA_FORM_STREAMS if few else _abi.PA_FORM_TILES), splits
+    each of `units` kv heads (pairs of them in the differential forms), cache rows
+    of `width` elements. Sequences whose rows a stream's columns hold on average
+    stream; the splits fill the chip once."""
+    form = _abi.PA_FORM_TILES
+    for few in (_abi.PA_FORM_STREAMS16, _abi.PA_FORM_STREAMS):
+        if rows * maps <= _COLUMNS[few] * batch:
+            form = few
+            break
+    work = max(1, max(batch, rows * maps // _COLUMNS[form]) * units)
+    slots = _PER_CU[form].get(width, 2) * cus
+    splits = 1
+    if work < SPLIT_BELOW * slots:
+        splits = max(1, min(-(-slots // work), -(-longest // MIN_SPLIT_TOKENS), _abi.PA_MAX_SPLITS))
+    return form, splits
 
 
 def _attend(fn_name, maps, q, cache, start, out, sm_scale, num_splits, max_seq_len, lam=None, norm_weight=None,
@@ -110,7 +119,7 @@ def _attend(fn_name, maps, q, cache, start, out, sm_scale, num_splits, max_seq_l
         return out
     capacity = blocks * cache.block_size
     longest = capacity if max_seq_len is None else max(0, min(int(max_seq_len), capacity))
-    form, planned = _plan(n * (hq // hkv), b, hkv // maps, longest, _cu_count(q.device), maps)
+    form, planned = _plan(n * (hq // hkv), b, hkv // maps, longest, _cu_count(q.device), maps * d, maps)
     num_splits = planned if num_splits is None else int(num_splits)
     po = pl = None
     if num_splits > 1:

@@ -15,12 +15,13 @@ from test_gpu_prefill import KV, case, offsets
 pytestmark = pytest.mark.gpu
 
 
-@pytest.fixture(autouse=True, params=["planned", "tiles", "streams"])
+@pytest.fixture(autouse=True, params=["planned", "tiles", "streams", "streams16"])
 def form(request, monkeypatch):
-    """Every test as the plan has it, and in the form for many rows and the one for few."""
+    """Every test as the plan has it, and in the form for many rows and the two for few."""
     if request.param != "planned":
         plan = prefill._plan
-        code = {"tiles": _abi.PA_FORM_TILES, "streams": _abi.PA_FORM_STREAMS}[request.param]
+        code = {"tiles": _abi.PA_FORM_TILES, "streams": _abi.PA_FORM_STREAMS,
+                "streams16": _abi.PA_FORM_STREAMS16}[request.param]
         monkeypatch.setattr(prefill, "_plan", lambda *a: (code, plan(*a)[1]))
     return request.param
 
