@@ -343,7 +343,7 @@ int pa_decode_pairs(const pa_decode_args *args, int *out);
 /* How the rows of a (sequence, kv head) are cut into workgroups; every form is
  * right for any number of them. A row is a new token and a query head of the kv
  * head's group; differential rows hold both maps, so a workgroup takes half as many. */
-#define PA_FORM_TILES 0     /* 128 rows: many rows a sequence */
+#define PA_FORM_TILES 0     /* 128 or 256 rows: many rows a sequence */
 #define PA_FORM_STREAMS 1   /* 32 rows, the waves share them and split the tokens: few */
 #define PA_FORM_STREAMS16 2 /* the same with 16 rows: fewer still */
 typedef struct pa_prefill_args {

@@ -44,29 +44,38 @@
 
 namespace {
 
+// Waves of a workgroup, two on a SIMD. Rows of 128 elements on: eight of one
+// workgroup, which share the loads, the staging registers and the LDS of a tile
+// (against two workgroups of four: a prompt of 16,384 tokens, 32 q / 8 kv heads
+// 2,380 -> 2,235 us; pairs of 128-element heads do not fit two waves otherwise, 505
+// -> 270 us for 4,096 tokens). Heads of 256: four, their accumulators and q take a
+// SIMD's registers.
+template <int D, int MAPS> constexpr int kTileWaves = D * MAPS >= 128 && D < 256 ? 8 : 4;
+
 // Compile-time geometry: MAPS maps of head_dim D each, a cache row of W = MAPS *
 // D elements, which is also the width of the value.
 template <int KV, int D, int MAPS>
 struct PGeo {
   static constexpr int W = D * MAPS;
   static constexpr int kElem = (KV == PA_KV_FP16 || KV == PA_KV_BF16) ? 2 : 1;
+  static constexpr int kNW = kTileWaves<D, MAPS>;       // waves of a workgroup
   static constexpr int BN = W <= 128 ? 64 : 32;         // tokens of a tile
   static constexpr int kPieceBytes = W * kElem >= 64 ? 16 : 8;  // of a lane's load
   static constexpr int kPieceElems = kPieceBytes / kElem;
   static constexpr int kPieceWords = kPieceBytes / 4;
   static constexpr int kPPR = W / kPieceElems;          // pieces of a row: 4 .. 32
-  static constexpr int kIter = BN * kPPR / (64 * kWaves);
+  static constexpr int kIter = BN * kPPR / (64 * kNW);
   // Rows padded so that 16 lanes reading 16 bytes of 16 rows (K), or four rows
   // of 64 bytes read transposed (V), use all 64 banks once.
   static constexpr int kKStride = W * 2 + 16;
   static constexpr int kVStride = W == 32 ? 64 : W * 2 + 64;
   static constexpr int kKBytes = BN * kKStride;
   static constexpr int kBufBytes = kKBytes + BN * kVStride;
-  static constexpr int kRowTile = kRowsPerWave * kWaves / MAPS;
+  static constexpr int kRowTile = kRowsPerWave * kNW / MAPS;
   static constexpr int kKSteps = D / 16;
   static constexpr int kDB = W / 32;  // 32-element blocks of the value
-  static constexpr int kWavesPerEU = W == 256 ? 1 : 2;
-  static_assert(64 / kPPR <= 16 && BN * kPPR % (64 * kWaves) == 0, "a wave's load lies in one page");
+  static constexpr int kWavesPerEU = D == 256 ? 1 : 2;
+  static_assert(64 / kPPR <= 16 && BN * kPPR % (64 * kNW) == 0, "a wave's load lies in one page");
 };
 
 template <int KV, int SC, int D, int MAPS>
@@ -95,7 +104,7 @@ struct LaneAddr {
 template <int KV, int D, int MAPS>
 __device__ __forceinline__ int first_row(int wave, int i) {
   using G = PGeo<KV, D, MAPS>;
-  return (64 * wave + 64 * kWaves * i) / G::kPPR;
+  return (64 * wave + 64 * G::kNW * i) / G::kPPR;
 }
 
 // The pages of the tile at n0 that this wave loads from. Rows past the sequence
@@ -278,8 +287,77 @@ __device__ __forceinline__ void add_wild(RowState<D, W> &st, const uint8_t *v, i
   }
 }
 
+// The sum over the wave, in every lane (all lanes active): adds across a row of 16
+// lanes by DPP, then of the rows' last lanes into the next rows.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+
+__device__ __forceinline__ int wave_sum(int x) {
+  x = dpp_add<0x111, 0xf>(x);  // row_shr:1
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);  // row_bcast:15 into rows 1 and 3
+  x = dpp_add<0x143, 0xc>(x);  // row_bcast:31 into rows 2 and 3
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
+// The row tile of this rank, longest first: a launch of a few rounds of workgroups
+// otherwise ends with whatever long tiles come last, alone on their CUs. Tile i of
+// sequence b sees about o_b + i row tiles' worth of tokens, o_b those before its new
+// ones, so count(x) = sum_b clamp(o_b + c_b - x, 0, c_b) tiles see x or more, and a
+// search over x finds the rank's level, one sequence a lane. Beyond 64 sequences:
+// in reverse order, so each sequence's longest come first. False: no such tile.
+template <int ROWS>
+__device__ __forceinline__ bool pick_tile(const PParams &p, int rank, int lane, int &b, int &index) {
+  if (!p.start) {
+    b = div_by(rank, p.by_seq_tiles);
+    index = rank - b * p.by_seq_tiles.d;
+    return true;
+  }
+  if (p.batch > 64) {
+    // sequence b's tiles are numbered from start_b * group / rows + b on: at
+    // least as many as it needs
+    auto key = [&](int start, int seq) { return (int)((uint32_t)(start * p.group) / ROWS) + seq; };
+    const int tile = p.tiles - 1 - rank;
+    b = find_sequence(p, tile, lane, key);
+    index = tile - key(row_start(p, b), b);
+    return index >= 0;
+  }
+  int c = 0, o = 0;
+  if (lane < p.batch) {
+    const int n = max(row_start(p, lane + 1) - row_start(p, lane), 0);
+    c = (n * p.group + ROWS - 1) / ROWS;
+    const int len = max(0, min(ro(p.seq_lens)[lane], p.max_tokens));
+    o = (int)min((int64_t)max(len - n, 0) * p.group / ROWS, (int64_t)1 << 24);
+  }
+  if (rank >= wave_sum(c)) return false;
+  // count(lo) > rank >= count(hi) = above, hi the first power of two past all tiles
+  int lo = 0, hi = 1, above = 0;
+  while (__builtin_amdgcn_ballot_w64(c > 0 && o + c > hi)) hi *= 2;
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    const int n = wave_sum(min(max(o + c - mid, 0), c));
+    if (n > rank) {
+      lo = mid;
+    } else {
+      hi = mid;
+      above = n;
+    }
+  }
+  uint64_t m = __builtin_amdgcn_ballot_w64(c > 0 && o <= lo && lo < o + c);
+  for (int k = rank - above; k > 0; --k) m &= m - 1;
+  b = __builtin_ctzll(m | (1ull << 63));
+  b = __builtin_amdgcn_readfirstlane(b);
+  index = lo - __builtin_amdgcn_readlane(o, b);
+  return true;
+}
+
 template <int KV, int SC, int D, int MAPS>
-__global__ void __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(PGeo<KV, D, MAPS>::kWavesPerEU)))
+__global__ void __launch_bounds__((64 * kTileWaves<D, MAPS>))
+    __attribute__((amdgpu_waves_per_eu(PGeo<KV, D, MAPS>::kWavesPerEU)))
 paged_prefill_kernel(const PParams p) {
   using G = PGeo<KV, D, MAPS>;
   constexpr int W = G::W;
@@ -294,27 +372,16 @@ paged_prefill_kernel(const PParams p) {
 
   // blockIdx = (split * tiles + tile) * units + unit: the units (kv heads) of the
   // same tokens run together, and with 8 of them each XCD keeps one head's K/V in
-  // its L2. Tiles go from the last, which see the most tokens. Splits are
+  // its L2. Row tiles go from those that see the most tokens on. Splits are
   // outermost: the later ones hold tokens of the longest sequences only, and a CU
   // that the round-robin gave always the same split would have all or no work
   // (24 sequences of 500-8,000 tokens in 4 splits 85.7 us, in 3 65.1).
   const uint32_t x1 = div_by(blockIdx.x, p.by_units);
   const int unit = blockIdx.x - x1 * p.units;
   const int split = div_by(x1, p.by_tiles);
-  const int tile = p.tiles - 1 - (int)(x1 - (uint32_t)split * p.tiles);
-
+  const int rank = x1 - (uint32_t)split * p.tiles;
   int b, index;
-  if (p.start) {
-    // sequence b's tiles are numbered from start_b * group / rows + b on: at
-    // least as many as it needs
-    auto key = [&](int start, int seq) { return (int)((uint32_t)(start * p.group) / G::kRowTile) + seq; };
-    b = find_sequence(p, tile, lane, key);
-    index = tile - key(row_start(p, b), b);
-    if (index < 0) return;
-  } else {
-    b = div_by(tile, p.by_seq_tiles);
-    index = tile - b * p.by_seq_tiles.d;
-  }
+  if (!pick_tile<G::kRowTile>(p, rank, lane, b, index)) return;
   const RowTile rt = tile_at<G::kRowTile>(p, b, index);
   if (rt.row0 >= rt.rows) return;
 
@@ -335,6 +402,7 @@ paged_prefill_kernel(const PParams p) {
   const int token = div_by((uint32_t)r, p.by_group);
   const int head = MAPS * (unit * p.group + (r - token * p.group)) + map;  // query head
   const int lim = rt.first + token;
+  const bool busy = rt.row0 + wave_row < rt.rows;  // the wave has rows; otherwise it only helps to load
   // the fewest tokens that a row of the wave sees
   const int least = rt.first + (int)div_by((uint32_t)min(rt.row0 + wave_row, rt.rows - 1), p.by_group) + 1;
   const int least_all = rt.first + (int)div_by((uint32_t)rt.row0, p.by_group) + 1;
@@ -359,7 +427,7 @@ paged_prefill_kernel(const PParams p) {
     const int piece = lane % G::kPPR;
     const int col = piece * G::kPieceElems;
 #pragma unroll
-    for (int i = 0; i < G::kIter; ++i) la.row[i] = (64 * kWaves * i + (int)threadIdx.x) / G::kPPR;
+    for (int i = 0; i < G::kIter; ++i) la.row[i] = (64 * G::kNW * i + (int)threadIdx.x) / G::kPPR;
     const uint32_t in_load = (uint32_t)lane / G::kPPR;
     const uint32_t part = (uint32_t)col / D;  // the differential cache row's half
     la.off = in_load * p.skt + part * p.skh + ((uint32_t)col - part * D) * G::kElem;
@@ -391,15 +459,17 @@ paged_prefill_kernel(const PParams p) {
         load(n0 + G::BN);
         load_pages<KV, D, MAPS>(page, p, bt_row, n0 + 2 * G::BN, rt.len, wave);
       }
-      const uint8_t *buf = sm + cur * G::kBufBytes;
-      f32x16 s[G::BN / 32];
-      scores_of<G::kKSteps, G::kKStride>(s, st.q, buf + k_lane);
-      if (n0 + G::BN > least) {
-        asm volatile("");  // a branch: as selects these would run on every tile
-        mask(s, n0, lim, h);
+      if (busy) {
+        const uint8_t *buf = sm + cur * G::kBufBytes;
+        f32x16 s[G::BN / 32];
+        scores_of<G::kKSteps, G::kKStride>(s, st.q, buf + k_lane);
+        if (n0 + G::BN > least) {
+          asm volatile("");  // a branch: as selects these would run on every tile
+          mask(s, n0, lim, h);
+        }
+        rescale(st, top_score(s, p.qk_scale));
+        accumulate<G::kVStride>(st, s, buf + G::kKBytes, v_lane, p.qk_scale);
       }
-      rescale(st, top_score(s, p.qk_scale));
-      accumulate<G::kVStride>(st, s, buf + G::kKBytes, v_lane, p.qk_scale);
       if (more && store_tile<KV, SC, D, MAPS>(sm + (cur ^ 1) * G::kBufBytes, staged, la, col, n0 + 2 * G::BN > least_all))
         sm_wild = 1;
       __syncthreads();
@@ -413,7 +483,7 @@ paged_prefill_kernel(const PParams p) {
         load(n0);
         store_tile<KV, SC, D, MAPS>(sm, staged, la, col, false);
         __syncthreads();
-        if (n0 + G::BN > least_all) add_wild<G::BN, G::kVStride>(st, sm + G::kKBytes, n0, lim, lane);
+        if (busy && n0 + G::BN > least_all) add_wild<G::BN, G::kVStride>(st, sm + G::kKBytes, n0, lim, lane);
         __syncthreads();
       }
     }
@@ -427,32 +497,66 @@ paged_prefill_kernel(const PParams p) {
   }
   // (a row that sees nothing is zeros; one whose visible scores are all -inf is 0 / 0)
   float inv = lim < 0 ? 0.f : 1.0f / l;
+  // Results leave through LDS: lanes hold eight bytes of 32 different rows, and
+  // stored so every 64 bytes of a row would be written in pieces.
+  auto store_result = [&](float f, bool normed) {
+    constexpr int kStride = W * 2 + 16, kLanes = W / 8, kRows = 64 / kLanes;
+    static_assert(G::kNW / MAPS * 32 * kStride <= 2 * G::kBufBytes, "the rows fit the tiles' LDS");
+    uint8_t *rows = sm + (wave / MAPS) * 32 * kStride;
+    const float *norm = normed ? p.norm : nullptr;
+#pragma unroll
+    for (int e = 0; e < W / 2; e += 4) {
+      const int d = 2 * e + 4 * h;
+      f32x4 y = {element(e) * f, element(e + 1) * f, element(e + 2) * f, element(e + 3) * f};
+      if (norm) y *= *reinterpret_cast<const f32x4 *>(norm + d);
+      store4(rows + (lane & 31) * kStride + 2 * d, y.x, y.y, y.z, y.w, p.io_bf16);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int i = 0; i < 32 / kRows; ++i) {
+      const int in_wave = i * kRows + lane / kLanes, at = rt.row0 + wave_row + in_wave;
+      if (at < rt.rows) {
+        const int tok = div_by((uint32_t)at, p.by_group), out_head = unit * p.group + (at - tok * p.group);
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(rows + in_wave * kStride + 16 * (lane % kLanes));
+        *reinterpret_cast<u32x4 *>(p.out + 2 * ((int64_t)(rt.token0 + tok) * p.sot + (int64_t)out_head * p.soh) +
+                                   16 * (lane % kLanes)) = x;
+      }
+    }
+  };
   if constexpr (MAPS == 1) {
-    if (live) store_rows<W, 32>(p, element, inv, false, rt.token0 + token, head, lane);
+    store_result(inv, false);
   } else {
-    float *other = reinterpret_cast<float *>(sm) + (wave / 2) * (W / 2) * 64;
-    __syncthreads();  // every wave is done with the tiles
-    if (map == 1) {
-      inv *= p.lam[(int64_t)(head / 2) * p.slam];
+    // the second map's waves hand theirs over, as many registers at a time as LDS holds
+    constexpr int kRegs = W / 2, kRounds = kRegs * G::kNW / 2 * 256 > 2 * G::kBufBytes ? 2 : 1, kPart = kRegs / kRounds;
+    static_assert(kPart * G::kNW / 2 * 256 <= 2 * G::kBufBytes, "a part fits the tiles' LDS");
+    float *other = reinterpret_cast<float *>(sm) + (wave / 2) * kPart * 64 + lane;
+    if (map == 1) inv *= p.lam[(int64_t)(head / 2) * p.slam];
+    float sq = 0.f;
 #pragma unroll
-      for (int d = 0; d < G::kDB; ++d)
+    for (int part = 0; part < kRounds; ++part) {
+      __syncthreads();  // every wave is done with the tiles, or with the part before
+      if (map == 1) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) other[(16 * d + i) * 64 + lane] = st.acc[d][i] * inv;
+        for (int e = 0; e < kPart; ++e) other[e * 64] = element(part * kPart + e) * inv;
+      }
+      __syncthreads();
+      if (map == 0) {
+#pragma unroll
+        for (int e = 0; e < kPart; ++e) {
+          const int i = part * kPart + e;
+          const float x = st.acc[i / 16][i % 16] * inv - other[e * 64];
+          st.acc[i / 16][i % 16] = x;
+          sq += x * x;
+        }
+      }
     }
     __syncthreads();
     if (map == 1) return;
-    float sq = 0.f;
-#pragma unroll
-    for (int d = 0; d < G::kDB; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        st.acc[d][i] = st.acc[d][i] * inv - other[(16 * d + i) * 64 + lane];
-        sq += st.acc[d][i] * st.acc[d][i];
-      }
     sq = half_sum(sq);
-    if (!live) return;
     const float f = p.norm ? __builtin_amdgcn_rsqf(sq * (1.0f / W) + p.norm_eps) * p.out_scale : 1.0f;
-    store_rows<W, 32>(p, element, f, true, rt.token0 + token, head / 2, lane);
+    store_result(f, true);
   }
 }
 
@@ -530,7 +634,7 @@ int build(const pa_prefill_args *a, int maps, PParams *out) {
   const int group = a->num_q_heads / a->num_kv_heads;
   const int units = a->num_kv_heads / maps;
   if ((int64_t)a->num_tokens * a->num_q_heads >= 2 * gib) return pa_fail(PA_ERR_UNSUPPORTED, "num_tokens * num_q_heads must be below 2^31");
-  const int columns = a->form == PA_FORM_TILES ? kRowsPerWave * kWaves : a->form == PA_FORM_STREAMS ? 32 : 16;
+  const int columns = a->form == PA_FORM_TILES ? kRowsPerWave * (d * maps >= 128 && d < 256 ? 8 : 4) : a->form == PA_FORM_STREAMS ? 32 : 16;
   const int row_tile = columns / maps;
   const int seq_tiles = (group + row_tile - 1) / row_tile;
   const int64_t tiles = a->query_start_loc ? (int64_t)a->num_tokens * group / row_tile + a->batch
@@ -591,7 +695,7 @@ template <int KV, int SC, int D, int MAPS>
 hipError_t launch(const PParams &p, hipStream_t st) {
   using G = PGeo<KV, D, MAPS>;
   hipLaunchKernelGGL((paged_prefill_kernel<KV, SC, D, MAPS>), dim3((uint32_t)(p.tiles * p.units * p.num_splits)),
-                     dim3(64 * kWaves), 0, st, p);
+                     dim3(64 * G::kNW), 0, st, p);
   if (p.num_splits > 1) launch_merge<G::W, MAPS, G::kRowTile>(p, st);
   return hipGetLastError();
 }

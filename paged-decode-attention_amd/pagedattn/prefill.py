@@ -19,10 +19,14 @@ from .hip_decode import _IO_CODE, _KV_CODE, _SCALE_CODE, _STORE_DTYPE, _cu_count
 
 # Columns of a workgroup's score products, by form (csrc/paged_prefill.hip,
 # csrc/paged_stream.hip): rows, a row being a new token and a head of its kv head's
-# group; the differential forms take two columns a row, one for each map.
+# group; the differential forms take two columns a row, one for each map. Tiles
+# have 256 where a cache row (of a pair, in the differential forms) has 128 elements
+# or more, unless a head has 256.
 _COLUMNS = {_abi.PA_FORM_TILES: 128, _abi.PA_FORM_STREAMS: 32, _abi.PA_FORM_STREAMS16: 16}
-# Workgroups that a CU holds at once, by form and elements of a cache row.
-_PER_CU = {_abi.PA_FORM_TILES: {256: 1}, _abi.PA_FORM_STREAMS: {256: 1}, _abi.PA_FORM_STREAMS16: {256: 2, 128: 4}}
+WIDE_TILE_COLUMNS = 256
+# Workgroups that a CU holds at once, by form and elements of a cache row (2 elsewhere).
+_PER_CU = {_abi.PA_FORM_TILES: {256: 1, 128: 1}, _abi.PA_FORM_STREAMS: {256: 1},
+           _abi.PA_FORM_STREAMS16: {256: 2, 128: 4}}
 # A split is a multiple of this many tokens; fewer than MIN_SPLIT_TOKENS are not
 # worth a partial and its share of the merge.
 MIN_SPLIT_TOKENS = 256
@@ -40,7 +44,10 @@ def _plan(rows: int, batch: int, units: int, longest: int, cus: int, width: int,
         if rows * maps <= _COLUMNS[few] * batch:
             form = few
             break
-    work = max(1, max(batch, rows * maps // _COLUMNS[form]) * units)
+    columns = _COLUMNS[form]
+    if form == _abi.PA_FORM_TILES and width >= 128 and width // maps < 256:
+        columns = WIDE_TILE_COLUMNS
+    work = max(1, max(batch, rows * maps // columns) * units)
     slots = _PER_CU[form].get(width, 2) * cus
     splits = 1
     if work < SPLIT_BELOW * slots:
