@@ -14,11 +14,14 @@
 // hold, every row that needs a page. The sums run over what was asked, so no row
 // overtakes an earlier one, and no atomics: the same inputs give the same tables.
 //
-// One workgroup sums the rows, 1,024 at a time, and moves the pages: page j of
-// all that move belongs to the row whose range of the sums holds j (a binary
-// search in LDS), so one long prompt does not hold up a lane. Slots are
-// independent of each other: a second launch writes them over the whole chip, or,
-// up to kSlotsInline of them, the same workgroup, which saves that launch.
+// One workgroup sums the rows, a chunk of its threads at a time. A row that moves
+// few pages and gets few tokens is written by its own thread, which has all it needs
+// in registers (the decode step: no search, three dependent loads in all); the
+// others go on a list in LDS that the waves share, a row a wave, so a long prompt
+// does not hold up a lane. With more than kSlotsInline tokens the slots are written
+// by a second launch over the whole chip, a binary search of the offsets each. What
+// bounds it is latency: the launch, the chain of loads, the prefix sums (three, by
+// DPP inside a wave).
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -29,10 +32,10 @@
 
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
-constexpr int kSlotsInline = 4096;
+constexpr int kSlotsInline = 16384;
 constexpr int kSlotThreads = 256;
+constexpr int kSearchRows = 4096;  // offsets that the slots' launch holds in LDS
+constexpr int kFew = 4;            // pages, tokens that a row's own thread writes
 
 struct TParams {
   int32_t *table;
@@ -55,28 +58,43 @@ __device__ __forceinline__ int pages_of(const TParams &p, int tokens) {
   return (int)div_by((uint32_t)tokens + (uint32_t)p.page - 1u, p.by_page);
 }
 
-// Exclusive prefix sums over the workgroup's threads; `total` gets the sum.
-template <typename T>
-__device__ __forceinline__ T block_scan(T x, T *wave_sums, T &total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T s = x;
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const T y = __shfl_up(s, o);
-    if (lane >= o) s += y;
-  }
+// x plus the value that DPP control CTRL hands the lanes of ROWS.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t dpp_add(int64_t x) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, false);
+  return x + (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
+}
+
+__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)x, lane), hi = __builtin_amdgcn_readlane((int)(x >> 32), lane);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// Exclusive prefix sums over the workgroup's threads; `total` gets the sum. Two
+// 32-bit sums fit one value, the upper one's addends shifted.
+template <int THREADS>
+__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t *wave_sums, int64_t &total) {
+  constexpr int kWaves = THREADS / 64;
+  static_assert(kWaves <= 16, "the waves' sums are added across a row of 16 lanes");
+  int64_t s = x;
+  s = dpp_add<0x111, 0xf>(s);  // row_shr:1
+  s = dpp_add<0x112, 0xf>(s);
+  s = dpp_add<0x114, 0xf>(s);
+  s = dpp_add<0x118, 0xf>(s);
+  s = dpp_add<0x142, 0xa>(s);  // row_bcast:15 into rows 1 and 3
+  s = dpp_add<0x143, 0xc>(s);  // row_bcast:31 into rows 2 and 3
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   __syncthreads();  // (an earlier scan's sums have been read)
   if (lane == 63) wave_sums[wave] = s;
   __syncthreads();
-  T before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const T t = wave_sums[w];
-    if (w < wave) before += t;
-    total += t;
-  }
-  return before + s - x;
+  int64_t w = lane < kWaves ? wave_sums[lane] : 0;
+  w = dpp_add<0x111, 0xf>(w);
+  w = dpp_add<0x112, 0xf>(w);
+  w = dpp_add<0x114, 0xf>(w);
+  w = dpp_add<0x118, 0xf>(w);
+  total = lane_value(w, kWaves - 1);
+  return (wave > 0 ? lane_value(w, wave - 1) : 0) + s - x;
 }
 
 // The last of n ascending values (the first at or below x) that is at or below x.
@@ -95,11 +113,8 @@ __device__ __forceinline__ int last_at_or_below(PTR v, int n, int x) {
   return lo;
 }
 
-// Slot and position of packed token i of row b.
-__device__ __forceinline__ void write_slot(const TParams &p, int i, int b, int row_start, int row_end) {
-  const int pos = p.lens_out[b] - (row_end - row_start) + (i - row_start);
-  const int blk = (int)div_by((uint32_t)pos, p.by_page);
-  p.slots[i] = (int64_t)p.table[b * p.stride + blk] * p.page + (pos - blk * p.page);
+__device__ __forceinline__ void write_slot(const TParams &p, int64_t i, int page, int pos, int blk) {
+  p.slots[i] = (int64_t)page * p.page + (pos - blk * p.page);
   if (p.positions) p.positions[i] = pos;
 }
 
@@ -108,97 +123,144 @@ __device__ __forceinline__ void write_pad(const TParams &p, int i) {
   if (p.positions) p.positions[i] = 0;
 }
 
-template <bool SLOTS>
-__global__ void __launch_bounds__(kThreads) step_rows_kernel(const TParams p) {
-  __shared__ int32_t sums[kWaves];
-  __shared__ int64_t wide_sums[kWaves];
-  __shared__ int32_t first[kThreads];  // this chunk's pages moved before row i
-  __shared__ int32_t at[kThreads];     // and the first column that they go to
-  const int tid = threadIdx.x;
+// A row that waves work on: its columns from `have` on take stack[from - 0, 1, ...]
+// (finished rows: give theirs to stack[from + 0, 1, ...]), its tokens go to packed
+// places from `begin` on.
+struct Job {
+  int32_t row, len, n, begin, have, need, from;
+};
+
+template <int THREADS, bool SLOTS>
+__global__ void __launch_bounds__(THREADS) step_rows_kernel(const TParams p) {
+  constexpr int kWaves = THREADS / 64;
+  __shared__ int64_t sums[kWaves];
+  __shared__ Job jobs[THREADS];
+  __shared__ int job_count;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int top = max(0, min(*p.count, p.stack_size));
   const int most = (int)min((int64_t)p.blocks * p.page, (int64_t)0x7fffffff);
+  if (tid == 0) job_count = 0;  // (the scans' barriers come before its first use)
 
   if (p.finished) {
-    for (int base = 0; base < p.rows; base += kThreads) {
+    for (int base = 0; base < p.rows; base += THREADS) {
       const int b = base + tid;
       int push = 0;
       if (b < p.rows && p.finished[b]) push = min(pages_of(p, min(max(p.lens[b], 0), most)), p.blocks);
-      int total;
-      first[tid] = block_scan(push, sums, total);
+      int64_t total;
+      const int first = (int)block_scan<THREADS>(push, sums, total);
+      if (push > 0) jobs[atomicAdd(&job_count, 1)] = Job{b, 0, 0, 0, 0, push, first};
       __syncthreads();
-      for (int j = tid; j < total; j += kThreads) {
-        const int r = last_at_or_below(first, kThreads, j);
-        const int64_t to = (int64_t)top + j;
-        if (to < p.stack_size) p.stack[to] = p.table[(base + r) * p.stride + (j - first[r])];
+      const int count = job_count;
+      for (int k = wave; k < count; k += kWaves) {
+        const Job j = jobs[k];
+        for (int c = lane; c < j.need; c += 64) {
+          const int64_t to = (int64_t)top + j.from + c;
+          if (to < p.stack_size) p.stack[to] = p.table[j.row * p.stride + c];
+        }
       }
+      __syncthreads();  // (also: what is pushed is seen by the pops below)
+      if (tid == 0) job_count = 0;
       top = (int)min((int64_t)top + total, (int64_t)p.stack_size);
-      __syncthreads();
     }
   }
 
-  int64_t asked = 0;          // tokens asked for before this chunk
+  int64_t asked = 0;                     // tokens asked for before this chunk
   int needed = 0, given = 0, taken = 0;  // pages needed, tokens given, pages taken before it
-  for (int base = 0; base < p.rows; base += kThreads) {
+  for (int base = 0; base < p.rows; base += THREADS) {
     const int b = base + tid;
-    int len = 0, n = 0;
+    int len = 0, n = 0, last = 0;
     if (b < p.rows) {
       len = p.finished && p.finished[b] ? 0 : max(p.lens[b], 0);
       n = max(p.fresh[b], 0);
+      // the page that the row's next token may share with its last
+      if constexpr (SLOTS) last = p.table[b * p.stride + min((int)div_by((uint32_t)min(len, most), p.by_page), p.blocks - 1)];
     }
     if ((int64_t)len + n > most) n = 0;
-    int64_t all;
-    const int64_t tokens_before = asked + block_scan<int64_t>(n, wide_sums, all);
-    asked += all;
+    int64_t total;
+    const int64_t tokens_before = asked + block_scan<THREADS>(n, sums, total);
+    asked += total;
     if (tokens_before + n > p.max_tokens) n = 0;
     const int have = pages_of(p, min(len, most));
     int need = pages_of(p, min(len, most) + n) - have;
-    int total;
-    const int pages_before = needed + block_scan(need, sums, total);
-    needed += total;
+    const int pages_before = needed + (int)block_scan<THREADS>(need, sums, total);
+    needed += (int)total;
     if (need > 0 && pages_before + need > top) n = need = 0;
-    const int begin = given + block_scan(n, sums, total);
-    given += total;
+    const int64_t both = block_scan<THREADS>((int64_t)need << 32 | n, sums, total);
+    const int begin = given + (int)both;
+    const int from = top - 1 - taken - (int)(both >> 32);
     if (b < p.rows) {
       p.start[b] = begin;
       p.lens_out[b] = len + n;
       if (b == p.rows - 1) p.start[p.rows] = begin + n;
     }
-    first[tid] = block_scan(need, sums, total);
-    at[tid] = have;
-    __syncthreads();
-    for (int j = tid; j < total; j += kThreads) {
-      const int r = last_at_or_below(first, kThreads, j);
-      p.table[(base + r) * p.stride + at[r] + (j - first[r])] = p.stack[top - 1 - taken - j];
+    if (need > kFew || (SLOTS && n > kFew)) {
+      jobs[atomicAdd(&job_count, 1)] = Job{b, len, n, begin, have, need, from};
+    } else if (need > 0 || n > 0) {
+      int page[kFew];
+#pragma unroll
+      for (int c = 0; c < kFew; ++c)
+        if (c < need) page[c] = p.stack[from - c];
+#pragma unroll
+      for (int c = 0; c < kFew; ++c)
+        if (c < need) p.table[b * p.stride + have + c] = page[c];
+      if constexpr (SLOTS) {
+#pragma unroll
+        for (int i = 0; i < kFew; ++i)
+          if (i < n) {
+            const int pos = len + i, blk = (int)div_by((uint32_t)pos, p.by_page);
+            int pg = last;
+#pragma unroll
+            for (int c = 0; c < kFew; ++c)
+              if (blk == have + c) pg = page[c];
+            write_slot(p, begin + i, pg, pos, blk);
+          }
+      }
     }
-    taken += total;
     __syncthreads();
+    const int count = job_count;
+    for (int k = wave; k < count; k += kWaves) {
+      const Job j = jobs[k];
+      int32_t *row = p.table + j.row * p.stride;
+      for (int c = lane; c < j.need; c += 64) row[j.have + c] = p.stack[j.from - c];
+      if constexpr (SLOTS) {
+        for (int i = lane; i < j.n; i += 64) {
+          const int pos = j.len + i, blk = (int)div_by((uint32_t)pos, p.by_page);
+          write_slot(p, j.begin + i, blk < j.have ? row[blk] : p.stack[j.from - (blk - j.have)], pos, blk);
+        }
+      }
+    }
+    given += (int)total;
+    taken += (int)(total >> 32);
+    __syncthreads();
+    if (tid == 0) job_count = 0;
   }
   if (tid == 0) {
     *p.count_out = top - taken;
     if (p.rows == 0) p.start[0] = 0;
   }
   if constexpr (SLOTS) {
-    // (the barrier above ends the writes of start, lens_out and table by this workgroup)
-    for (int i = tid; i < p.max_tokens; i += kThreads) {
-      if (i < given) {
-        const int b = last_at_or_below(p.start, p.rows, i);
-        write_slot(p, i, b, p.start[b], p.start[b + 1]);
-      } else {
-        write_pad(p, i);
-      }
-    }
+    for (int i = given + tid; i < p.max_tokens; i += THREADS) write_pad(p, i);
   }
 }
 
 __global__ void __launch_bounds__(kSlotThreads) step_slots_kernel(const TParams p) {
+  __shared__ int32_t starts[kSearchRows];
   const int i = blockIdx.x * kSlotThreads + threadIdx.x;
-  if (i >= p.max_tokens) return;
-  if (i < p.start[p.rows]) {
-    const int b = last_at_or_below(p.start, p.rows, i);
-    write_slot(p, i, b, p.start[b], p.start[b + 1]);
-  } else {
-    write_pad(p, i);
+  const bool in_lds = p.rows <= kSearchRows;
+  if (in_lds) {
+    for (int b = threadIdx.x; b < p.rows; b += kSlotThreads) starts[b] = p.start[b];
+    __syncthreads();
   }
+  if (i >= p.max_tokens) return;
+  if (i >= p.start[p.rows]) {
+    write_pad(p, i);
+    return;
+  }
+  const int b = in_lds ? last_at_or_below(starts, p.rows, i) : last_at_or_below(p.start, p.rows, i);
+  const int begin = p.start[b];
+  const int pos = p.lens_out[b] - (p.start[b + 1] - begin) + (i - begin);
+  const int blk = (int)div_by((uint32_t)pos, p.by_page);
+  write_slot(p, i, p.table[b * p.stride + blk], pos, blk);
 }
 
 }  // namespace
@@ -249,12 +311,14 @@ extern "C" int pa_step_tables(const pa_step_tables_args *a, void *stream) {
   p.stride = a->stride_btb;
   p.by_page = make_div((uint32_t)a->block_size);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (p.max_tokens <= kSlotsInline) {
-    hipLaunchKernelGGL((step_rows_kernel<true>), dim3(1), dim3(kThreads), 0, st, p);
-  } else {
-    hipLaunchKernelGGL((step_rows_kernel<false>), dim3(1), dim3(kThreads), 0, st, p);
+  // few rows: few waves to add up
+  const bool small = p.rows <= 256, inlined = p.max_tokens <= kSlotsInline;
+  if (small && inlined) hipLaunchKernelGGL((step_rows_kernel<256, true>), dim3(1), dim3(256), 0, st, p);
+  else if (inlined) hipLaunchKernelGGL((step_rows_kernel<1024, true>), dim3(1), dim3(1024), 0, st, p);
+  else if (small) hipLaunchKernelGGL((step_rows_kernel<256, false>), dim3(1), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((step_rows_kernel<1024, false>), dim3(1), dim3(1024), 0, st, p);
+  if (!inlined)
     hipLaunchKernelGGL(step_slots_kernel, dim3((p.max_tokens + kSlotThreads - 1) / kSlotThreads), dim3(kSlotThreads), 0, st, p);
-  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return pa_fail(PA_ERR_HIP, "launch failed: %s", hipGetErrorString(e));
   return pa_ok();

@@ -238,3 +238,21 @@ def test_serving_run():
     assert int(count) == pool - held
     owned = [p for b in range(rows) for p in table[b, :-(-len(said[b]) // page)].tolist()]
     assert sorted(owned + free[:int(count)].tolist()) == list(range(pool))
+
+
+@pytest.mark.parametrize("rows", [3, 257, 1500])
+@pytest.mark.parametrize("max_tokens", [16384, 16385, 40000])
+def test_between_one_launch_and_two(rows, max_tokens):
+    """Rows of one to a few pages and of many, in turn, around the size that takes a second launch."""
+    r = random.Random(rows + max_tokens)
+    lens = [r.choice([0, 1, 15, 16, 17, 100, 900]) for _ in range(rows)]
+    new = [r.choice([0, 1, 2, 4, 5, 16, 64, 65, 81, 130]) for _ in range(rows)]
+    pages = [-(-x // 16) for x in lens]
+    pool = list(range(sum(pages) + sum(new) // 8 + rows))
+    r.shuffle(pool)
+    size = len(pool)
+    table = [[pool.pop() for _ in range(n)] + [0] * (70 - n) for n in pages]
+    stack = pool + [0] * (size - len(pool))
+    gone = [r.random() < 0.3 for _ in range(rows)]
+    check(table, lens, new, stack, len(pool), 16, max_tokens)
+    check(table, lens, new, stack, len(pool), 16, max_tokens, gone, in_place=True)
