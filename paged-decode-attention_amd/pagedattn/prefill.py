@@ -55,9 +55,68 @@ def _plan(rows: int, batch: int, units: int, longest: int, cus: int, width: int,
     return form, splits
 
 
+# Checked argument structs by the geometry they were checked for: shapes, strides,
+# types and devices of every tensor and the call's numbers, nothing of a tensor's
+# identity or address. A call of a known geometry copies its struct and sets the
+# pointers (the C side checks every call again).
+_CHECKED: dict[tuple, tuple] = {}
+_CHECKED_MAX = 512
+_copy_args = _abi.PaPrefillArgs.from_buffer_copy
+
+
 def _attend(fn_name, maps, q, cache, start, out, sm_scale, num_splits, max_seq_len, lam=None, norm_weight=None,
             norm_eps=0.0, out_scale=1.0):
-    """Validate a call's tensors, pack pa_prefill_args and launch."""
+    """Check a call's tensors (once per geometry), fill pa_prefill_args and launch."""
+    k, v, ks, vs, bt, sl = (cache.k_cache, cache.v_cache, cache.k_scale, cache.v_scale, cache.block_table,
+                            cache.seq_lens)
+    shape = cache.shape
+    # (numbers by value: a tensor given as one would be a key by its identity)
+    sm_scale = None if sm_scale is None else float(sm_scale)
+    num_splits = None if num_splits is None else int(num_splits)
+    max_seq_len = None if max_seq_len is None else int(max_seq_len)
+    norm_eps, out_scale = float(norm_eps), float(out_scale)
+    key = (fn_name, q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(),
+           v.shape, v.stride(), v.dtype, v.get_device(), bt.shape, bt.stride(), bt.dtype, bt.get_device(),
+           sl.shape, sl.stride(), sl.dtype, sl.get_device(), cache.kv_dtype, cache.block_size, shape.num_q_heads,
+           shape.num_kv_heads, shape.head_dim, sm_scale, num_splits, max_seq_len, norm_eps, out_scale)
+    for t in (start, out, lam, norm_weight, ks, vs):
+        key += (None,) if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+    hit = _CHECKED.get(key)
+    if hit is None:
+        hit = _check(maps, q, cache, start, out, sm_scale, num_splits, max_seq_len, lam, norm_weight, norm_eps,
+                     out_scale)
+        if len(_CHECKED) >= _CHECKED_MAX:
+            _CHECKED.clear()
+        _CHECKED[key] = hit
+    args, out_shape, part_out, part = hit
+    if out is None:
+        out = torch.empty(out_shape, dtype=q.dtype, device=q.device)
+    if args is None:  # no rows
+        return out
+    a = _copy_args(args)
+    a.q, a.k_cache, a.v_cache, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+    a.block_table, a.seq_lens = bt.data_ptr(), sl.data_ptr()
+    if start is not None:
+        a.query_start_loc = start.data_ptr()
+    if lam is not None:
+        a.lam = lam.data_ptr()
+        if norm_weight is not None:
+            a.norm_weight = norm_weight.data_ptr()
+    if cache.kv_dtype == "int8":
+        a.k_scale, a.v_scale = ks.data_ptr(), vs.data_ptr()
+    if part:
+        partials = torch.empty((part,), dtype=torch.float32, device=q.device)
+        a.part_out = partials.data_ptr()
+        a.part_lse = a.part_out + part_out
+    rc = _launch(q, getattr(_abi.load(), fn_name), a)
+    if rc:
+        _abi.check(rc, fn_name)
+    return out
+
+
+def _check(maps, q, cache, start, out, sm_scale, num_splits, max_seq_len, lam, norm_weight, norm_eps, out_scale):
+    """(struct without pointers or None where there are no rows, the result's shape,
+    bytes of part_out, floats of all partials) of a call, or the error of a wrong one."""
     if q.dim() != 3:
         raise ValueError(f"q {tuple(q.shape)} is not [tokens, heads, head_dim]")
     n, hq, d = q.shape
@@ -71,13 +130,9 @@ def _attend(fn_name, maps, q, cache, start, out, sm_scale, num_splits, max_seq_l
         raise ValueError(f"q has {hq} heads of {d}, cache shape expects {shape.num_q_heads} of {shape.head_dim}")
     if hkv <= 0 or hq % hkv or hkv % maps:
         raise ValueError(f"{hq} query heads and {hkv} kv heads do not group" + (" in pairs" if maps == 2 else ""))
-    if not q.is_cuda:
-        raise ValueError(f"q is on {q.device}: the HIP kernel needs GPU tensors")
     k, v, bt, sl = cache.k_cache, cache.v_cache, cache.block_table, cache.seq_lens
     out_shape = (n, hq // maps, maps * d)
-    if out is None:
-        out = torch.empty(out_shape, dtype=q.dtype, device=q.device)
-    elif out.shape != out_shape or out.dtype != q.dtype:
+    if out is not None and (out.shape != out_shape or out.dtype != q.dtype):
         raise ValueError(f"out {out.dtype} {tuple(out.shape)} is not {q.dtype} {out_shape}")
     dev = q.get_device()
     for name, t in (("k_cache", k), ("v_cache", v), ("out", out), ("block_table", bt), ("seq_lens", sl),
@@ -86,8 +141,9 @@ def _attend(fn_name, maps, q, cache, start, out, sm_scale, num_splits, max_seq_l
             raise ValueError(f"{name} is on {t.device}, q on {q.device}")
     if k.dtype != _STORE_DTYPE[kv_dtype] or v.dtype != k.dtype:
         raise ValueError(f"k/v cache dtype {k.dtype}/{v.dtype} does not match kv_dtype {kv_dtype}")
-    kst, qst, ost = k.stride(), q.stride(), out.stride()
-    if tuple(k.shape[1:]) != (cache.block_size, hkv, d) or v.shape != k.shape or v.stride() != kst:
+    kst, qst = k.stride(), q.stride()
+    ost = (out_shape[1] * out_shape[2], out_shape[2], 1) if out is None else out.stride()
+    if k.dim() != 4 or tuple(k.shape[1:]) != (cache.block_size, hkv, d) or v.shape != k.shape or v.stride() != kst:
         raise ValueError(f"k_cache {tuple(k.shape)} is not [NB, {cache.block_size}, {hkv}, {d}], or v_cache differs")
     if kst[3] != 1 or (qst[2] != 1 and n) or (ost[2] != 1 and n):
         raise ValueError("head_dim must be the contiguous (stride-1) dimension of q, out and the caches")
@@ -101,7 +157,6 @@ def _attend(fn_name, maps, q, cache, start, out, sm_scale, num_splits, max_seq_l
             raise ValueError(f"q has {n} rows for {b} sequences")
     elif start.dtype != torch.int32 or start.shape != (b + 1,) or (b and start.stride(0) != 1):
         raise ValueError(f"query_start_loc must be contiguous int32 [{b + 1}]")
-    ks = vs = None
     sst, scale_code = (0, 0), _abi.PA_SCALE_NONE
     if kv_dtype == "int8":
         ks, vs = cache.k_scale, cache.v_scale
@@ -113,7 +168,7 @@ def _attend(fn_name, maps, q, cache, start, out, sm_scale, num_splits, max_seq_l
                              "head dimension")
         if ks.get_device() != dev or vs.get_device() != dev:
             raise ValueError("scales must live on q's device")
-        scale_code, ks, vs = _SCALE_CODE[ks.dtype], ks.data_ptr(), vs.data_ptr()
+        scale_code = _SCALE_CODE[ks.dtype]
     lam_stride = 0
     if maps == 2:
         if lam.dtype != torch.float32 or lam.shape != (hq // 2,):
@@ -122,31 +177,28 @@ def _attend(fn_name, maps, q, cache, start, out, sm_scale, num_splits, max_seq_l
         if norm_weight is not None and (norm_weight.dtype != torch.float32 or norm_weight.shape != (2 * d,)
                                         or norm_weight.stride(0) != 1):
             raise ValueError(f"norm_weight must be contiguous float32 [{2 * d}]")
+    if not q.is_cuda:
+        raise ValueError(f"q is on {q.device}: the HIP kernel needs GPU tensors")
     if n == 0 or b == 0:
-        return out
+        return None, out_shape, 0, 0
     capacity = blocks * cache.block_size
-    longest = capacity if max_seq_len is None else max(0, min(int(max_seq_len), capacity))
+    longest = capacity if max_seq_len is None else max(0, min(max_seq_len, capacity))
     form, planned = _plan(n * (hq // hkv), b, hkv // maps, longest, _cu_count(q.device), maps * d, maps)
-    num_splits = planned if num_splits is None else int(num_splits)
-    po = pl = None
-    if num_splits > 1:
-        part = torch.empty((num_splits * n * hq * (maps * d + 1),), dtype=torch.float32, device=q.device)
-        po = part.data_ptr()
-        pl = po + 4 * num_splits * n * hq * maps * d
-    args = _abi.PaPrefillArgs(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), ks, vs, out.data_ptr(), po, pl, bt.data_ptr(), sl.data_ptr(),
-        None if start is None else start.data_ptr(), None if lam is None else lam.data_ptr(),
-        None if norm_weight is None else norm_weight.data_ptr(),
-        b, n, hq, hkv, d, cache.block_size, k.shape[0], blocks, num_splits,
-        0 if max_seq_len is None else longest, form,
-        qst[0], qst[1], kst[0], kst[1], kst[2], sst[0], sst[1], ost[0], ost[1],
-        bt.stride(0) if b > 1 else blocks, lam_stride,
-        _KV_CODE[kv_dtype], scale_code, _IO_CODE[q.dtype], d ** -0.5 if sm_scale is None else float(sm_scale),
-        float(norm_eps), float(out_scale))
-    rc = _launch(q, getattr(_abi.load(), fn_name), args)
-    if rc:
-        _abi.check(rc, fn_name)
-    return out
+    num_splits = planned if num_splits is None else num_splits
+    rows = num_splits * n * hq if num_splits > 1 else 0
+    args = _abi.PaPrefillArgs()
+    args.batch, args.num_tokens, args.num_q_heads, args.num_kv_heads, args.head_dim = b, n, hq, hkv, d
+    args.block_size, args.num_blocks, args.max_blocks = cache.block_size, k.shape[0], blocks
+    args.num_splits, args.max_seq_len, args.form = num_splits, 0 if max_seq_len is None else longest, form
+    args.stride_qt, args.stride_qh = qst[0], qst[1]
+    args.stride_kn, args.stride_kt, args.stride_kh = kst[0], kst[1], kst[2]
+    args.stride_sn, args.stride_st = sst[0], sst[1]
+    args.stride_ot, args.stride_oh = ost[0], ost[1]
+    args.stride_btb, args.stride_lam = bt.stride(0) if b > 1 else blocks, lam_stride
+    args.kv_dtype, args.scale_dtype, args.io_dtype = _KV_CODE[kv_dtype], scale_code, _IO_CODE[q.dtype]
+    args.sm_scale = d ** -0.5 if sm_scale is None else sm_scale
+    args.norm_eps, args.out_scale = norm_eps, out_scale
+    return args, out_shape, 4 * rows * maps * d, rows * (maps * d + 1)
 
 
 def paged_prefill_hip(

@@ -28,15 +28,37 @@ class StepTables:
     free_count: torch.Tensor       # [1] int32: pages left on the stack
 
 
-def _vector(name: str, t: torch.Tensor, n: int | None, dtype: torch.dtype, device: torch.device) -> int:
-    """The address of a contiguous 1-D tensor of n elements (None: any number)."""
-    if t.dtype != dtype or t.dim() != 1 or (n is not None and t.shape[0] != n):
-        raise ValueError(f"{name} must be {dtype} [{'n' if n is None else n}], got {t.dtype} {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, block_table on {device}")
-    return t.data_ptr()
+# Geometries (shapes, strides, types, devices) that have been checked; nothing of a
+# tensor's identity or address.
+_CHECKED: set[tuple] = set()
+_CHECKED_MAX = 512
+
+
+def _check(block_table, vectors, max_tokens) -> None:
+    if block_table.dtype != torch.int32 or block_table.dim() != 2:
+        raise ValueError(f"block_table must be int32 [B, max_blocks], got {block_table.dtype} "
+                         f"{tuple(block_table.shape)}")
+    dev = block_table.device
+    b, blocks = block_table.shape
+    if blocks < 1 or (blocks > 1 and b and block_table.stride(1) != 1):
+        raise ValueError("block_table rows must be contiguous and not empty")
+    if max_tokens < 0:
+        raise ValueError(f"max_tokens {max_tokens} < 0")
+    sizes = {"seq_lens": b, "new_lens": b, "finished": b, "free_pages": None, "free_count": 1, "seq_lens_out": b,
+             "free_count_out": 1, "query_start_loc": b + 1, "slot_mapping": max_tokens, "positions": max_tokens}
+    types = {"finished": torch.bool, "slot_mapping": torch.int64, "positions": torch.int64}
+    for (name, n), t in zip(sizes.items(), vectors):
+        if t is None:
+            continue
+        dtype = types.get(name, torch.int32)
+        if t.dtype != dtype or t.dim() != 1 or (n is not None and t.shape[0] != n):
+            raise ValueError(f"{name} must be {dtype} [{'n' if n is None else n}], got {t.dtype} {tuple(t.shape)}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, block_table on {dev}")
+    if dev.type != "cuda":
+        raise ValueError(f"block_table is on {dev}: the tables are built on the GPU")
 
 
 def build_step_tables(
@@ -72,41 +94,37 @@ def build_step_tables(
     owns its pages: pages shared between rows must not be returned through
     `finished`.
     """
-    if block_table.dtype != torch.int32 or block_table.dim() != 2:
-        raise ValueError(f"block_table must be int32 [B, max_blocks], got {block_table.dtype} "
-                         f"{tuple(block_table.shape)}")
-    dev = block_table.device
-    if dev.type != "cuda":
-        raise ValueError(f"block_table is on {dev}: the tables are built on the GPU")
+    max_tokens, block_size = int(max_tokens), int(block_size)
+    # (outputs that are not given need no check)
+    vectors = (seq_lens, new_lens, finished, free_pages, free_count, seq_lens_out, free_count_out, query_start_loc,
+               slot_mapping, positions)
+    key = (block_table.shape, block_table.stride(), block_table.dtype, block_table.get_device(), max_tokens,
+           *[None if t is None else (t.shape, t.dtype, t.get_device(), t.is_contiguous()) for t in vectors])
+    if key not in _CHECKED:
+        _check(block_table, vectors, max_tokens)
+        if len(_CHECKED) >= _CHECKED_MAX:
+            _CHECKED.clear()
+        _CHECKED.add(key)
     b, blocks = block_table.shape
-    if blocks < 1 or (blocks > 1 and block_table.stride(1) != 1):
-        raise ValueError("block_table rows must be contiguous and not empty")
-    if max_tokens < 0:
-        raise ValueError(f"max_tokens {max_tokens} < 0")
     if seq_lens_out is None:
         seq_lens_out = seq_lens
     if free_count_out is None:
         free_count_out = free_count
+    dev = block_table.device
     if query_start_loc is None:
         query_start_loc = torch.empty((b + 1,), dtype=torch.int32, device=dev)
-    if slot_mapping is None:
+    if slot_mapping is None and positions is None:
+        slot_mapping, positions = torch.empty((2, max_tokens), dtype=torch.int64, device=dev).unbind(0)
+    elif slot_mapping is None:
         slot_mapping = torch.empty((max_tokens,), dtype=torch.int64, device=dev)
-    if positions is None:
+    elif positions is None:
         positions = torch.empty((max_tokens,), dtype=torch.int64, device=dev)
-    i32, i64 = torch.int32, torch.int64
     args = _abi.PaStepTablesArgs(
-        block_table.data_ptr(),
-        _vector("seq_lens", seq_lens, b, i32, dev),
-        _vector("new_lens", new_lens, b, i32, dev),
-        None if finished is None else _vector("finished", finished, b, torch.bool, dev),
-        _vector("free_pages", free_pages, None, i32, dev),
-        _vector("free_count", free_count, 1, i32, dev),
-        _vector("seq_lens_out", seq_lens_out, b, i32, dev),
-        _vector("free_count_out", free_count_out, 1, i32, dev),
-        _vector("query_start_loc", query_start_loc, b + 1, i32, dev),
-        _vector("slot_mapping", slot_mapping, max_tokens, i64, dev),
-        _vector("positions", positions, max_tokens, i64, dev),
-        b, blocks, block_size, free_pages.shape[0], max_tokens, block_table.stride(0) if b > 1 else blocks)
+        block_table.data_ptr(), seq_lens.data_ptr(), new_lens.data_ptr(),
+        None if finished is None else finished.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
+        seq_lens_out.data_ptr(), free_count_out.data_ptr(), query_start_loc.data_ptr(), slot_mapping.data_ptr(),
+        positions.data_ptr(), b, blocks, block_size, free_pages.shape[0], max_tokens,
+        block_table.stride(0) if b > 1 else blocks)
     rc = _launch(block_table, _abi.load().pa_step_tables, args)
     if rc:
         _abi.check(rc, "pa_step_tables")

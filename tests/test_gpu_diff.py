@@ -23,6 +23,7 @@ def form(request, monkeypatch):
         code = {"tiles": _abi.PA_FORM_TILES, "streams": _abi.PA_FORM_STREAMS,
                 "streams16": _abi.PA_FORM_STREAMS16}[request.param]
         monkeypatch.setattr(prefill, "_plan", lambda *a: (code, plan(*a)[1]))
+    monkeypatch.setattr(prefill, "_CHECKED", {})  # (what is kept there has its form)
     return request.param
 
 THIN = ModelShape(12, 4, 32, "thin")
