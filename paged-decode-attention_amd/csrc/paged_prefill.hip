@@ -148,28 +148,34 @@ __device__ __forceinline__ void load_tile(Staged<KV, SC, D, MAPS> &st, const PPa
 
 // The staged tile into an LDS buffer (K rows, then V rows). With `tame`,
 // infinities and NaN of V become zeros, and the result tells whether this lane
-// had one.
+// had one. int8: the scales of K's MAPS heads, then V's, into `scales`.
 template <int KV, int SC, int D, int MAPS>
 __device__ __forceinline__ bool store_tile(uint8_t *buf, const Staged<KV, SC, D, MAPS> &st, const LaneAddr &la,
-                                           int col, bool tame) {
+                                           int col, bool tame, float *scales) {
   using G = PGeo<KV, D, MAPS>;
   constexpr int kHalves = G::kPieceElems / 2;  // words
   bool wild = false;
 #pragma unroll
   for (int i = 0; i < G::kIter; ++i) {
     uint32_t h[kHalves];
-    to_halves<KV, SC>(h, st.k[i], KV == PA_KV_INT8 ? st.ks[KV == PA_KV_INT8 ? i : 0] : 0);
+    to_halves<KV>(h, st.k[i]);
     uint8_t *kd = buf + la.row[i] * G::kKStride + col * 2;
 #pragma unroll
     for (int w = 0; w < kHalves; w += 4) *reinterpret_cast<u32x4 *>(kd + 4 * w) = u32x4{h[w], h[w + 1], h[w + 2], h[w + 3]};
-    to_halves<KV, SC>(h, st.v[i], KV == PA_KV_INT8 ? st.vs[KV == PA_KV_INT8 ? i : 0] : 0);
-    if (tame) {
+    to_halves<KV>(h, st.v[i]);
+    if (KV != PA_KV_INT8 && tame) {
 #pragma unroll
       for (int w = 0; w < kHalves; ++w) wild |= tame_word(h[w]);
     }
     uint8_t *vd = buf + G::kKBytes + la.row[i] * G::kVStride + col * 2;
 #pragma unroll
     for (int w = 0; w < kHalves; w += 4) *reinterpret_cast<u32x4 *>(vd + 4 * w) = u32x4{h[w], h[w + 1], h[w + 2], h[w + 3]};
+    if constexpr (KV == PA_KV_INT8) {
+      if (col % D == 0) {
+        scales[col / D * G::BN + la.row[i]] = scale_value<SC>(st.ks[i]);
+        scales[(MAPS + col / D) * G::BN + la.row[i]] = finite_scale(scale_value<SC>(st.vs[i]));
+      }
+    }
   }
   return wild;
 }
@@ -178,8 +184,9 @@ template <int D, int W>
 struct RowState {
   f16x8 q[D / 16];
   f32x16 acc[W / 32];
-  float m;  // running maximum (log2 domain), -inf before the first visible score
+  float m;  // running maximum - kTopLog2 (log2 domain), -inf before the first visible score
   float l;  // sum over this lane's tokens
+  float limit;  // int8: the accumulators' unit (raise_limit)
 };
 
 // Scores of a tile's tokens: lane (row = lane & 31, half h) holds those of tokens
@@ -221,9 +228,9 @@ __device__ __forceinline__ float top_score(const f32x16 (&s)[NB], float qk_scale
 // Moves the running maximum to `top` where that is far above it.
 template <int D, int W>
 __device__ __forceinline__ void rescale(RowState<D, W> &st, float top) {
-  const bool need = top > st.m + kRescaleLog2;
+  const bool need = top > st.m + (kTopLog2 + kRescaleLog2);
   if (__builtin_expect(__builtin_amdgcn_ballot_w64(need) != 0, 0)) {
-    const float m_new = need ? top : st.m;
+    const float m_new = need ? top - kTopLog2 : st.m;
     const float alpha = need ? __builtin_amdgcn_exp2f(st.m - m_new) : 1.0f;
     st.l *= alpha;
 #pragma unroll
@@ -234,9 +241,10 @@ __device__ __forceinline__ void rescale(RowState<D, W> &st, float top) {
 
 // Scores to P, and O^T += V^T P^T, 16 tokens a product: lane (row d = lane & 31, half
 // h) holds tokens 16 kb + 8 (j / 4) + 4 h + j % 4 of V^T, as the scores lie.
-template <int VSTRIDE, int D, int W, int NB>
+// int8 (PARTS > 0: heads of a value row): times V's scales in `vs`, over the limit.
+template <int VSTRIDE, int PARTS, int D, int W, int NB>
 __device__ __forceinline__ void accumulate(RowState<D, W> &st, f32x16 (&s)[NB], const uint8_t *v, uint32_t v_lane,
-                                           float qk_scale) {
+                                           float qk_scale, const float *vs, int h) {
   // (a row that has seen nothing yet: every score is -inf and P is 0)
   const float m = st.m == -INFINITY ? 0.f : st.m;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -248,18 +256,50 @@ __device__ __forceinline__ void accumulate(RowState<D, W> &st, f32x16 (&s)[NB], 
       sum[i & 3] += s[b][i];
     }
   st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  constexpr int kHeads = PARTS > 0 ? PARTS : 1;
+  float inv = 1.f;
+  if constexpr (PARTS > 0) {
+    float top = 0.f;
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+      for (int e = 0; e < 16 * NB; e += 4) {
+        const f32x4 v4 = *reinterpret_cast<const f32x4 *>(vs + 32 * NB * part + score_token<32>(e, h));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(s[e / 16][e % 16 + j] * v4[j]));
+      }
+    bool any;
+    const float f = raise_limit<32>(st.limit, top, any);
+    if (__builtin_expect(any, 0)) {
+#pragma unroll
+      for (int d = 0; d < W / 32; ++d) st.acc[d] *= f;
+    }
+    inv = inverse_limit(st.limit);
+  }
 #pragma unroll
   for (int kb = 0; kb < 2 * NB; ++kb) {
-    uint32_t w[4];
+    f16x8 pop[kHeads];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f16x2 two = {(_Float16)s[kb / 2][8 * (kb & 1) + 2 * j], (_Float16)s[kb / 2][8 * (kb & 1) + 2 * j + 1]};
-      w[j] = __builtin_bit_cast(uint32_t, two);
+    for (int part = 0; part < kHeads; ++part) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = 8 * (kb & 1) + 2 * j;
+        float a = s[kb / 2][i], b = s[kb / 2][i + 1];
+        if constexpr (PARTS > 0) {
+          const float *at = vs + 32 * NB * part + score_token<32>(8 * kb + 2 * j, h);
+          a = a * at[0] * inv;  // (in this order: 0 times the largest scale is 0)
+          b = b * at[1] * inv;
+        }
+        const f16x2 two = {(_Float16)a, (_Float16)b};
+        w[j] = __builtin_bit_cast(uint32_t, two);
+      }
+      pop[part] = as_f16x8(w[0], w[1], w[2], w[3]);
     }
-    const f16x8 pop = as_f16x8(w[0], w[1], w[2], w[3]);
 #pragma unroll
     for (int d = 0; d < W / 32; ++d)
-      st.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(read_columns(v + 16 * kb * VSTRIDE + 64 * d + v_lane, 8 * VSTRIDE), pop, st.acc[d], 0, 0, 0);
+      st.acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+          read_columns(v + 16 * kb * VSTRIDE + 64 * d + v_lane, 8 * VSTRIDE), pop[d * kHeads / (W / 32)], st.acc[d], 0, 0, 0);
   }
 }
 
@@ -362,6 +402,9 @@ paged_prefill_kernel(const PParams p) {
   using G = PGeo<KV, D, MAPS>;
   constexpr int W = G::W;
   __shared__ __attribute__((aligned(16))) uint8_t sm[2 * G::kBufBytes];
+  constexpr bool kInt8 = KV == PA_KV_INT8;
+  constexpr int kTileScales = 2 * MAPS * G::BN;  // of K's heads, then of V's
+  __shared__ __attribute__((aligned(16))) float sm_sc[kInt8 ? 2 * kTileScales : 4];
   __shared__ int sm_wild;  // V holds an infinity or NaN in a masked tile
 
   const int lane = threadIdx.x & 63;
@@ -410,6 +453,7 @@ paged_prefill_kernel(const PParams p) {
   RowState<D, W> st;
   st.m = -INFINITY;
   st.l = 0.f;
+  st.limit = 0.f;
 #pragma unroll
   for (int d = 0; d < G::kDB; ++d) st.acc[d] = f32x16{};
   {
@@ -448,7 +492,7 @@ paged_prefill_kernel(const PParams p) {
     load(lo);
     load_pages<KV, D, MAPS>(page, p, bt_row, lo + G::BN, rt.len, wave);
     __syncthreads();  // (sm_wild)
-    if (store_tile<KV, SC, D, MAPS>(sm, staged, la, col, lo + G::BN > least_all)) sm_wild = 1;
+    if (store_tile<KV, SC, D, MAPS>(sm, staged, la, col, lo + G::BN > least_all, sm_sc)) sm_wild = 1;
     __syncthreads();
     const uint32_t k_lane = (lane & 31) * G::kKStride + map * D * 2 + 16 * h;
     const uint32_t v_lane = (4 * h + ((lane & 15) >> 2)) * G::kVStride + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
@@ -463,25 +507,30 @@ paged_prefill_kernel(const PParams p) {
         const uint8_t *buf = sm + cur * G::kBufBytes;
         f32x16 s[G::BN / 32];
         scores_of<G::kKSteps, G::kKStride>(s, st.q, buf + k_lane);
-        if (n0 + G::BN > least) {
+        const float *scales = sm_sc + (kInt8 ? cur * kTileScales : 0);
+        const bool masked = n0 + G::BN > least;
+        if constexpr (kInt8)
+          scale_scores<32, G::BN / 2>([&](int e, float k) { s[e / 16][e % 16] *= k; }, scales + map * G::BN, h);
+        if (masked) {
           asm volatile("");  // a branch: as selects these would run on every tile
           mask(s, n0, lim, h);
         }
         rescale(st, top_score(s, p.qk_scale));
-        accumulate<G::kVStride>(st, s, buf + G::kKBytes, v_lane, p.qk_scale);
+        accumulate<G::kVStride, kInt8 ? MAPS : 0>(st, s, buf + G::kKBytes, v_lane, p.qk_scale, scales + MAPS * G::BN, h);
       }
-      if (more && store_tile<KV, SC, D, MAPS>(sm + (cur ^ 1) * G::kBufBytes, staged, la, col, n0 + 2 * G::BN > least_all))
+      if (more && store_tile<KV, SC, D, MAPS>(sm + (cur ^ 1) * G::kBufBytes, staged, la, col, n0 + 2 * G::BN > least_all,
+                                              sm_sc + (kInt8 ? (cur ^ 1) * kTileScales : 0)))
         sm_wild = 1;
       __syncthreads();
       cur ^= 1;
     }
-    if (__builtin_expect(sm_wild, 0)) {
+    if (!kInt8 && __builtin_expect(sm_wild, 0)) {
       // the masked tiles once more, with V as it is
       const int from = max(lo, max(least_all - 1, 0) / G::BN * G::BN);
       for (int n0 = from; n0 < hi; n0 += G::BN) {
         load_pages<KV, D, MAPS>(page, p, bt_row, n0, rt.len, wave);
         load(n0);
-        store_tile<KV, SC, D, MAPS>(sm, staged, la, col, false);
+        store_tile<KV, SC, D, MAPS>(sm, staged, la, col, false, sm_sc);
         __syncthreads();
         if (busy && n0 + G::BN > least_all) add_wild<G::BN, G::kVStride>(st, sm + G::kKBytes, n0, lim, lane);
         __syncthreads();
@@ -490,6 +539,10 @@ paged_prefill_kernel(const PParams p) {
   }
 
   const float l = half_sum(st.l);
+  if constexpr (kInt8) {
+#pragma unroll
+    for (int d = 0; d < G::kDB; ++d) st.acc[d] *= st.limit;
+  }
   auto element = [&](int e) { return st.acc[e / 16][e % 16]; };
   if (!direct) {
     if (live) store_partial<W, 32>(p, element, st.m, l, split, rt.token0 + token, head, lane);

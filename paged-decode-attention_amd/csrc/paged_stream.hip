@@ -12,10 +12,11 @@
 // The maps of a differential row differ in the half of the K row they meet: every
 // column meets both halves, in sums of their own, and a lane keeps its map's.
 //
-// What bounds it is the stream of K and V. They take turns in a wave's LDS slot; each
-// is loaded again as soon as it is stored, a whole tile ahead. Rows of 512 bytes take
-// turns in the registers too (V on its way during K's products and the softmax, the
-// next tile's K during V's), which leaves room for a second wave on the SIMD.
+// What bounds it is the stream of K and V. They take turns in a wave's registers and
+// in its LDS slot: V is on its way during K's products and the softmax, the next
+// tile's K during V's. Half the registers and LDS so hold twice the waves, which keeps
+// as many bytes in flight as both at once and measured faster (160 int8 sequences of
+// 100 to 8,000 tokens 57 -> 52 us).
 // The loads are non-temporal: a step reads each byte once (64 sequences of 4,096
 // tokens, pairs of 128-element heads, fp16: 203 us with plain loads, 180 with these).
 // 16 columns where they hold the rows: the accumulators, the softmax and the
@@ -24,27 +25,6 @@
 #include "prefill_common.h"
 
 namespace {
-
-// x combined over the lanes that share a column.
-template <int COLS>
-__device__ __forceinline__ float column_max(float x) {
-  if constexpr (COLS == 16) {
-    const uint32_t u = __float_as_uint(x);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  }
-  return half_max(x);
-}
-
-template <int COLS>
-__device__ __forceinline__ float column_sum(float x) {
-  if constexpr (COLS == 16) {
-    const uint32_t u = __float_as_uint(x);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  }
-  return half_sum(x);
-}
 
 // For a lane of map 1, its value minus that of the same row's map 2, COLS / 2 lanes on.
 template <int COLS>
@@ -78,8 +58,6 @@ struct SGeo {
   static constexpr int kScores = COLS / 2;         // of a lane and tile
   static constexpr int kAcc = W * COLS / 64;       // accumulator floats of a lane
   static constexpr int kSteps = D * COLS / 512;    // score products of a map (16 or 32 elements each)
-  // Whether K and V take turns in the same registers (rows of 512 bytes).
-  static constexpr bool kTurns = true;
   static constexpr int kWavesPerEU = COLS == 16 ? (W == 256 ? 2 : 3) : W == 256 ? 1 : 2;
 };
 
@@ -127,6 +105,8 @@ paged_stream_kernel(const PParams p) {
   constexpr int kBytes = kWaves * G::kSlot > kAccBytes ? kWaves * G::kSlot : kAccBytes;
   __shared__ __attribute__((aligned(16))) uint8_t sm[kBytes];
   __shared__ float sm_m[kWaves][COLS], sm_l[kWaves][COLS];
+  constexpr bool kInt8 = KV == PA_KV_INT8;
+  __shared__ __attribute__((aligned(16))) float sm_sc[kInt8 ? kWaves * 2 * MAPS * 32 : 4];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -179,6 +159,7 @@ paged_stream_kernel(const PParams p) {
   const int64_t scale_off = (int64_t)unit * MAPS * (SC == PA_SCALE_FP32 ? 4 : 2);
   const ro_i32 *bt_row = ro(p.bt) + (int64_t)rt.b * p.sbtb;
   uint8_t *slot = sm + wave * G::kSlot;
+  float *k_scales = sm_sc + (kInt8 ? wave * 2 * MAPS * 32 : 0), *v_scales = k_scales + (kInt8 ? MAPS * 32 : 0);
 
   // the pages of the tile at n0 (a multiple of 32: each 16-token half lies in one)
   auto pages = [&](int n0, int (&pg)[2]) {
@@ -186,10 +167,9 @@ paged_stream_kernel(const PParams p) {
     for (int u = 0; u < 2; ++u) pg[u] = bt_row[(uint32_t)min(n0 + 16 * u, rt.len - 1) >> p.log2_page];
   };
   typedef Half<KV, G::kIter, G::kPieceWords> HalfTile;
-  HalfTile tk, own_v;
-  HalfTile &tv = G::kTurns ? tk : own_v;
+  HalfTile t;
   // rows at or past the sequence's end read as zeros
-  auto load = [&](HalfTile &t, const uint8_t *base, const uint8_t *sbase, int n0, const int (&pg)[2]) {
+  auto load = [&](const uint8_t *base, const uint8_t *sbase, int n0, const int (&pg)[2]) {
 #pragma unroll
     for (int i = 0; i < G::kIter; ++i) {
       const int r0 = i * (64 / G::kPPR);  // first row of the load
@@ -205,36 +185,41 @@ paged_stream_kernel(const PParams p) {
   };
   // into the wave's slot; with `tame`, infinities and NaN become zeros, and the
   // result tells whether this lane had one
-  auto store = [&](const HalfTile &t, int stride, bool tame) {
+  auto store = [&](int stride, bool tame, float *scales) {
     bool wild = false;
 #pragma unroll
     for (int i = 0; i < G::kIter; ++i) {
       constexpr int kHalves = G::kPieceElems / 2;
       uint32_t x[kHalves];
-      to_halves<KV, SC>(x, t.w[i], KV == PA_KV_INT8 ? t.scale[KV == PA_KV_INT8 ? i : 0] : 0);
-      if (tame) {
+      to_halves<KV>(x, t.w[i]);
+      if (!kInt8 && tame) {
 #pragma unroll
         for (int w = 0; w < kHalves; ++w) wild |= tame_word(x[w]);
       }
       uint8_t *d = slot + (i * (64 / G::kPPR) + row_in) * stride + ecol * 2;
 #pragma unroll
       for (int w = 0; w < kHalves; w += 4) *reinterpret_cast<u32x4 *>(d + 4 * w) = u32x4{x[w], x[w + 1], x[w + 2], x[w + 3]};
+      if constexpr (kInt8) {
+        const float sc = scale_value<SC>(t.scale[i]);
+        if (ecol % D == 0) scales[part * 32 + i * (64 / G::kPPR) + row_in] = scales == v_scales ? finite_scale(sc) : sc;
+      }
     }
     return wild;
   };
 
-  typename B::type acc[G::kAcc / B::kFloats] = {};
+  constexpr int kBlocks = G::kAcc / B::kFloats;  // of the value's elements
+  typename B::type acc[kBlocks] = {};
   auto element = [&](int e) -> float { return acc[e / B::kFloats][e % B::kFloats]; };
-  float m = -INFINITY;  // running maximum (log2 domain)
+  float m = -INFINITY;  // running maximum - kTopLog2 (log2 domain)
   float l = 0.f;        // sum over this lane's tokens
+  float limit = 0.f;    // int8: the accumulators' unit (raise_limit)
   f16x8 q[G::kSteps];
   bool wild = false;
   const int n_first = lo + 32 * wave;
   if (n_first < hi) {
     int pg[2];
     pages(n_first, pg);
-    load(tk, p.k, p.ks, n_first, pg);
-    if constexpr (!G::kTurns) load(tv, p.v, p.vs, n_first, pg);
+    load(p.k, p.ks, n_first, pg);
     const uint16_t *qrow = reinterpret_cast<const uint16_t *>(p.q) + (int64_t)(rt.token0 + token) * p.sqt +
                            (int64_t)head * p.sqh + 8 * grp;
 #pragma unroll
@@ -242,10 +227,8 @@ paged_stream_kernel(const PParams p) {
       const u32x4 w = *reinterpret_cast<const u32x4 *>(qrow + 8 * kGroups * ks);
       q[ks] = p.io_bf16 ? bf16x8_to_f16x8(w) : __builtin_bit_cast(f16x8, w);
     }
-    if constexpr (G::kTurns) {
-      store(tk, G::kKStride, false);
-      load(tv, p.v, p.vs, n_first, pg);
-    }
+    store(G::kKStride, false, k_scales);
+    load(p.v, p.vs, n_first, pg);
     pages(n_first + 32 * kWaves, pg);
     const uint8_t *k_lane = slot + col * G::kKStride + 16 * grp;
     // V: 16 lanes take four rows (4 * group on) of 16 columns
@@ -255,12 +238,7 @@ paged_stream_kernel(const PParams p) {
     for (int n0 = n_first; n0 < hi; n0 += 32 * kWaves) {
       const bool masked = n0 + 32 > least;
       const int next = n0 + 32 * kWaves;
-      if constexpr (!G::kTurns) {
-        store(tk, G::kKStride, false);
-        if (next < hi) load(tk, p.k, p.ks, next, pg);
-      }
       sync_slot();
-      // scores: element e is token 256 / COLS * (e / 4) + 4 * grp + e % 4
       float s[G::kScores];
 #pragma unroll
       for (int u = 0; u < 32 / COLS; ++u) {
@@ -274,19 +252,20 @@ paged_stream_kernel(const PParams p) {
 #pragma unroll
         for (int i = 0; i < B::kFloats; ++i) s[B::kFloats * u + i] = MAPS == 2 && map == 1 ? two[i] : one[i];
       }
+      if constexpr (kInt8) scale_scores<COLS, G::kScores>([&](int e, float k) { s[e] *= k; }, k_scales + 32 * map, grp);
       if (masked) {
         asm volatile("");  // a branch: as selects these would run on every tile
 #pragma unroll
         for (int e = 0; e < G::kScores; ++e)
-          if (n0 + 256 / COLS * (e / 4) + 4 * grp + e % 4 > lim) s[e] = -INFINITY;
+          if (n0 + score_token<COLS>(e, grp) > lim) s[e] = -INFINITY;
       }
       float top = s[0];
 #pragma unroll
       for (int e = 1; e < G::kScores; ++e) top = fmaxf(top, s[e]);
       top = column_max<COLS>(top) * p.qk_scale;
-      const bool need = top > m + kRescaleLog2;
+      const bool need = top > m + (kTopLog2 + kRescaleLog2);
       if (__builtin_expect(__builtin_amdgcn_ballot_w64(need) != 0, 0)) {
-        const float m_new = need ? top : m;
+        const float m_new = need ? top - kTopLog2 : m;
         const float alpha = need ? __builtin_amdgcn_exp2f(m - m_new) : 1.0f;
         l *= alpha;
 #pragma unroll
@@ -296,51 +275,93 @@ paged_stream_kernel(const PParams p) {
       // (a row that has seen nothing yet: every score is -inf and P is 0)
       const float base = m == -INFINITY ? 0.f : m;
       float sum[2] = {0.f, 0.f};
-      uint32_t w[G::kScores / 2];
 #pragma unroll
-      for (int e = 0; e < G::kScores; e += 2) {
-        const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], p.qk_scale, -base));
-        const float c = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 1], p.qk_scale, -base));
-        sum[0] += a;
-        sum[1] += c;
-        const f16x2 pair = {(_Float16)a, (_Float16)c};
-        w[e / 2] = __builtin_bit_cast(uint32_t, pair);
+      for (int e = 0; e < G::kScores; ++e) {
+        s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], p.qk_scale, -base));
+        sum[e & 1] += s[e];
       }
       l += sum[0] + sum[1];
       sync_slot();
-      wild |= store(tv, G::kVStride, masked);
+      wild |= store(G::kVStride, masked, v_scales);
       sync_slot();
-      if (next < hi) {
-        if constexpr (G::kTurns) {
-          load(tk, p.k, p.ks, next, pg);
-        } else {
-          load(tv, p.v, p.vs, next, pg);
-          pages(next + 32 * kWaves, pg);
+      if (next < hi) load(p.k, p.ks, next, pg);
+      // P as product operands; int8: by head of the value row, times V's scales.
+      // Differential rows, whose difference can be far smaller than its terms, take P as
+      // two fp16 values, cut to 11 bits and what that leaves: the stream has time for
+      // the second product, and P's rounding stays out of the result.
+      constexpr int kHeads = kInt8 ? MAPS : 1;
+      constexpr bool kTwice = MAPS == 2;
+      uint32_t cut[kHeads][G::kScores / 2], left[kHeads][G::kScores / 2];
+      float inv = 1.f;
+      if constexpr (kInt8) {
+        float top = 0.f;
+#pragma unroll
+        for (int part = 0; part < kHeads; ++part)
+#pragma unroll
+          for (int e = 0; e < G::kScores; e += 4) {
+            const f32x4 v4 = *reinterpret_cast<const f32x4 *>(v_scales + 32 * part + score_token<COLS>(e, grp));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(s[e + j] * v4[j]));
+          }
+        bool any;
+        const float f = raise_limit<COLS>(limit, top, any);
+        if (__builtin_expect(any, 0)) {
+#pragma unroll
+          for (int d = 0; d < kBlocks; ++d) acc[d] *= f;
         }
+        inv = inverse_limit(limit);
       }
+#pragma unroll
+      for (int part = 0; part < kHeads; ++part)
+#pragma unroll
+        for (int e = 0; e < G::kScores; e += 2) {
+          float a = s[e], c = s[e + 1];
+          if constexpr (kInt8) {
+            const float *at = v_scales + 32 * part + score_token<COLS>(e, grp);
+            a = a * at[0] * inv;  // (in this order: 0 times the largest scale is 0)
+            c = c * at[1] * inv;
+          }
+          if constexpr (kTwice) {
+            cut[part][e / 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, c));
+            const f16x2 h = __builtin_bit_cast(f16x2, cut[part][e / 2]);
+            const f16x2 r = {(_Float16)(a - (float)h[0]), (_Float16)(c - (float)h[1])};
+            left[part][e / 2] = __builtin_bit_cast(uint32_t, r);
+          } else {
+            const f16x2 h = {(_Float16)a, (_Float16)c};
+            cut[part][e / 2] = __builtin_bit_cast(uint32_t, h);
+          }
+        }
 #pragma unroll
       for (int kb = 0; kb < G::kScores / 8; ++kb) {
-        const f16x8 pop = as_f16x8(w[4 * kb], w[4 * kb + 1], w[4 * kb + 2], w[4 * kb + 3]);
+        f16x8 pop[kHeads], rest[kHeads];
+#pragma unroll
+        for (int part = 0; part < kHeads; ++part) {
+          pop[part] = as_f16x8(cut[part][4 * kb], cut[part][4 * kb + 1], cut[part][4 * kb + 2], cut[part][4 * kb + 3]);
+          if constexpr (kTwice)
+            rest[part] = as_f16x8(left[part][4 * kb], left[part][4 * kb + 1], left[part][4 * kb + 2], left[part][4 * kb + 3]);
+        }
         // 32 columns: tokens 16 kb + 8 (j / 4) + 4 grp + j % 4; 16: 16 (j / 4) + 4 grp + j % 4
 #pragma unroll
-        for (int d = 0; d < G::kAcc / B::kFloats; ++d)
-          acc[d] = B::product(read_columns(slot + 16 * kb * G::kVStride + 2 * COLS * d + v_lane, 256 / COLS * G::kVStride),
-                              pop, acc[d]);
+        for (int d = 0; d < kBlocks; ++d) {
+          const f16x8 v = read_columns(slot + 16 * kb * G::kVStride + 2 * COLS * d + v_lane, 256 / COLS * G::kVStride);
+          acc[d] = B::product(v, pop[d * kHeads / kBlocks], acc[d]);
+          if constexpr (kTwice) acc[d] = B::product(v, rest[d * kHeads / kBlocks], acc[d]);
+        }
       }
       sync_slot();
-      if (G::kTurns && next < hi) {
-        store(tk, G::kKStride, false);
-        load(tv, p.v, p.vs, next, pg);
+      if (next < hi) {
+        store(G::kKStride, false, k_scales);
+        load(p.v, p.vs, next, pg);
         pages(next + 32 * kWaves, pg);
       }
     }
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(wild) != 0, 0)) {
+    if (!kInt8 && __builtin_expect(__builtin_amdgcn_ballot_w64(wild) != 0, 0)) {
       // V's infinities and NaN in masked tiles, added to the rows that see them
       for (int n0 = n_first; n0 < hi; n0 += 32 * kWaves) {
         if (n0 + 32 <= least) continue;
         pages(n0, pg);
-        load(tv, p.v, p.vs, n0, pg);
-        store(tv, G::kVStride, false);
+        load(p.v, p.vs, n0, pg);
+        store(G::kVStride, false, v_scales);
         sync_slot();
         for (int t1 = 0; t1 < 32; ++t1) {
           const uint8_t *vrow = slot + t1 * G::kVStride + 8 * grp;
@@ -362,6 +383,10 @@ paged_stream_kernel(const PParams p) {
     }
   }
 
+  if constexpr (kInt8) {
+#pragma unroll
+    for (int d = 0; d < kBlocks; ++d) acc[d] *= limit;
+  }
   // join the waves
   const float lw = column_sum<COLS>(l);
   if (grp == 0) {

@@ -51,6 +51,10 @@ typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4;
 constexpr int kRowsPerWave = 32;
+// P is 2^kTopLog2 at the running maximum, which moves only when a score passes it by
+// kRescaleLog2: P stays below 2^15, in fp16's range, and what is far below the maximum
+// stays out of its subnormals for longer. (The sums hold the same factor.)
+constexpr float kTopLog2 = 7.0f;
 constexpr float kRescaleLog2 = 8.0f;
 constexpr int kSplitUnit = 128;  // splits are multiples of this many tokens
 // A lane offset past every buffer (page_rsrc's -1 leaves all others in range):
@@ -69,6 +73,75 @@ __device__ __forceinline__ float half_sum(float x) {
   const uint32_t u = __float_as_uint(x);
   const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// x combined over the 64 / COLS lanes that share a column.
+template <int COLS>
+__device__ __forceinline__ float column_max(float x) {
+  if constexpr (COLS == 16) {
+    const uint32_t u = __float_as_uint(x);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  }
+  return half_max(x);
+}
+
+template <int COLS>
+__device__ __forceinline__ float column_sum(float x) {
+  if constexpr (COLS == 16) {
+    const uint32_t u = __float_as_uint(x);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  }
+  return half_sum(x);
+}
+
+// Token (in its tile) of a lane's score e: four neighbouring tokens a lane group.
+template <int COLS>
+__device__ __forceinline__ int score_token(int e, int grp) {
+  return 256 / COLS * (e / 4) + 4 * grp + e % 4;
+}
+
+// int8: scores times their tokens' K scales (in LDS); multiply(e, k) takes k to score e.
+template <int COLS, int N, typename MULTIPLY>
+__device__ __forceinline__ void scale_scores(MULTIPLY multiply, const float *scales, int grp) {
+#pragma unroll
+  for (int e = 0; e < N; e += 4) {
+    const f32x4 k4 = *reinterpret_cast<const f32x4 *>(scales + score_token<COLS>(e, grp));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) multiply(e + j, k4[j]);
+  }
+}
+
+// int8: V's scale as P meets it before its rounding to fp16. Tokens that a row does
+// not see may have any scale and their P is 0: infinities and NaN become the largest
+// float, whose product with 0 is 0 and with any other P is fp16's infinity.
+__device__ __forceinline__ float finite_scale(float s) {
+  constexpr float kMost = 3.4028234663852886e38f;
+  return fminf(fmaxf(s, -kMost), kMost);
+}
+
+// So that neither large nor small products leave fp16's range they are divided by a
+// power of two, `limit` (0 before the first), which follows the largest product of
+// the lane's row so far, `top`, with room for 2^7 times that; the accumulators are in
+// units of it. Moves the limit up where `top` has passed its room, and returns what
+// the accumulators have to be multiplied by; nothing to do when no lane had to (`any`
+// false).
+template <int COLS>
+__device__ __forceinline__ float raise_limit(float &limit, float top, bool &any) {
+  top = column_max<COLS>(fminf(top, 0x1p100f));  // (an infinity makes the row's result one, at any limit)
+  const bool need = top > limit * 32768.f;
+  any = __builtin_amdgcn_ballot_w64(need) != 0;
+  if (__builtin_expect(!any, 1)) return 1.f;
+  const uint32_t e = max(__float_as_uint(top) >> 23, 30u);
+  const float f = need ? limit * __uint_as_float((261 - e) << 23) : 1.f;
+  if (need) limit = __uint_as_float((e - 7) << 23);
+  return f;
+}
+
+// 1 / limit, a power of two (0 where the row has met no product).
+__device__ __forceinline__ float inverse_limit(float limit) {
+  return limit > 0.f ? __uint_as_float((254u << 23) - __float_as_uint(limit)) : 0.f;
 }
 
 // First row of sequence b among the packed rows, kept inside them whatever the
@@ -146,9 +219,11 @@ __device__ __forceinline__ uint32_t load_scale(__amdgpu_buffer_rsrc_t r, uint32_
   else return __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
 }
 
-// A piece's elements as fp16 words (two elements each).
-template <int KV, int SC, int WORDS>
-__device__ __forceinline__ void to_halves(uint32_t *h, const uint32_t (&w)[WORDS], uint32_t scale_bits) {
+// A piece's elements as fp16 words (two elements each). int8 values come as they are,
+// exactly; their scales meet the scores and P (below), so no product is rounded to
+// fp16 on the way in.
+template <int KV, int WORDS>
+__device__ __forceinline__ void to_halves(uint32_t *h, const uint32_t (&w)[WORDS]) {
   if constexpr (KV == PA_KV_FP16) {
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) h[i] = w[i];
@@ -161,22 +236,24 @@ __device__ __forceinline__ void to_halves(uint32_t *h, const uint32_t (&w)[WORDS
       h[2 * i] = bytes_to_halves<KV>(w[i], w[i], pair_sel<KV>(0, 1));
       h[2 * i + 1] = bytes_to_halves<KV>(w[i], w[i], pair_sel<KV>(2, 3));
     }
-  } else if constexpr (SC == PA_SCALE_FP16) {
-    const uint32_t s2 = scale_bits | (scale_bits << 16);
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i) {
-      h[2 * i] = i8pair_fp16_scale(w[i] ^ kInt8Sign, 0, 1, s2);
-      h[2 * i + 1] = i8pair_fp16_scale(w[i] ^ kInt8Sign, 2, 3, s2);
-    }
   } else {
-    const float s = __uint_as_float(scale_bits) * kInt8Unit, c = s * (-1.0f / 131072.0f);
+    // x + 128 under the exponent byte 0x64 is 1024 + (x + 128)
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) {
       const uint32_t x = w[i] ^ kInt8Sign;
-      h[2 * i] = i8pair_fp32_scale(perm(x, x, pair_sel<KV>(0, 1)), s, c, s, c);
-      h[2 * i + 1] = i8pair_fp32_scale(perm(x, x, pair_sel<KV>(2, 3)), s, c, s, c);
+      const f16x2 a = __builtin_bit_cast(f16x2, perm(kF16Exp1024, x, 0x04010400u));
+      const f16x2 b = __builtin_bit_cast(f16x2, perm(kF16Exp1024, x, 0x04030402u));
+      const f16x2 c = {(_Float16)1152.0f, (_Float16)1152.0f};
+      h[2 * i] = __builtin_bit_cast(uint32_t, a - c);
+      h[2 * i + 1] = __builtin_bit_cast(uint32_t, b - c);
     }
   }
+}
+
+template <int SC>
+__device__ __forceinline__ float scale_value(uint32_t bits) {
+  if constexpr (SC == PA_SCALE_FP32) return __uint_as_float(bits);
+  else return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
 }
 
 // Whether a half of the word is an infinity or NaN.

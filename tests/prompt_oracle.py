@@ -1,11 +1,11 @@
 """Causal and differential paged attention in float64, with a bound on what the kernel may be off.
 
-Plain loops over sequences and heads, from the formulas; no code of the package but
-`dequantize_kv`, whose fp16 values are what the kernels attend over.
+Plain loops over sequences and heads, from the formulas. Cache rows are what they stand for: int8
+values times their scales exactly, bf16 rows as fp16 (the same value inside fp16's range).
 
 The bound, per output element, before the result's own rounding (half a step, u_out |y|):
-  * P is rounded to fp16 (2^-11 of p, or 2^-25 where it is subnormal; the row's normaliser is at
-    least 1): 2^-11 sum p|v| + 2^-25 sum |v|;
+  * P (int8: P times V's scale) is rounded to fp16 (2^-11 of p, or 2^-25 where it is subnormal;
+    the row's normaliser is at least 1): 2^-11 sum p|v| + 2^-25 sum |v|;
   * scores: D products summed in fp32 and one fma, D + 2 roundings of at most 2^-24 of sum |q k|
     each, twice (numerator and normaliser), and exp2 (2^-22);
   * sums over T tokens in fp32: T 2^-24, twice.
@@ -14,8 +14,6 @@ The bound, per output element, before the result's own rounding (half a step, u_
 from __future__ import annotations
 
 import torch
-
-from pagedattn.cache import dequantize_kv
 
 HALF_STEP = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 
@@ -28,8 +26,11 @@ def dense_rows(cache, b):
     off = pos % cache.block_size
     rows = []
     for store, scale in ((cache.k_cache, cache.k_scale), (cache.v_cache, cache.v_scale)):
-        s = None if scale is None else scale[blk, off]
-        rows.append(dequantize_kv(store[blk, off], s, cache.kv_dtype).double())
+        x = store[blk, off]
+        if scale is not None:
+            rows.append(x.double() * scale[blk, off].double()[..., None])
+        else:
+            rows.append(x.to(torch.float16).double())
     return rows
 
 

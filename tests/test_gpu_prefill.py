@@ -205,6 +205,38 @@ def test_infinities_reach_only_the_rows_that_see_them(junk, which, splits):
     # (an infinite K makes a score of +inf, NaN after the softmax, or of -inf, by the sign of q)
 
 
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("sdt", [torch.float16, torch.float32])
+def test_int8_scales_of_any_size(sdt, splits):
+    """Scales far apart, all tiny, all large, beyond what fp16 holds: P * scale stays in range."""
+    for seed, factors in enumerate(([1e-3, 1.0, 300.0], [1e-4], [2000.0], [0.0, 1.0])):
+        q, c, start = case(LLAMA3_8B, [9, 40], [600, 70], "int8", sdt, seed=60 + seed)
+        r = torch.Generator().manual_seed(seed)
+        pick = torch.tensor(factors)[torch.randint(len(factors), c.v_scale.shape, generator=r)].cuda()
+        c.v_scale.copy_(c.v_scale * pick)
+        check(q, c, start, num_splits=splits)
+    if sdt == torch.float32:
+        c.v_scale.mul_(1e7)
+        got = paged_prefill_hip(q.bfloat16(), c, offsets(start), num_splits=splits)
+        want, bound = po.attend(q.bfloat16(), c, start)
+        assert po.worst(got, want, bound) < 1
+
+
+@pytest.mark.parametrize("junk", [float("inf"), float("nan"), 1e30])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_int8_scales_reach_only_the_rows_that_see_them(junk, which, splits):
+    q, c, start = case(LLAMA3_8B, [150], [170], "int8", torch.float32, seed=70)
+    before = paged_prefill_hip(q, c, offsets(start), num_splits=splits).clone()
+    t = 20 + 77  # row 77's token
+    (c.k_scale if which == "k" else c.v_scale)[c.block_table[0, t // 16].long(), t % 16] = junk
+    got = paged_prefill_hip(q, c, offsets(start), num_splits=splits)
+    assert torch.equal(got[:77], before[:77])
+    if which == "v":
+        hit = got[77:].float()  # (a value of 0, or a P that rounds to it, may meet the scale)
+        assert float((~torch.isfinite(hit)).float().mean()) > 0.9
+
+
 def test_strides():
     """q cut out of packed q/k/v rows, out inside a wider buffer, the cache with heads outermost in the page."""
     shape = LLAMA3_8B
