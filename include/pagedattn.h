@@ -389,7 +389,9 @@ typedef struct pa_prefill_args {
 /* Causal paged GQA attention of the last n_b = query_start_loc[b + 1] -
  * query_start_loc[b] tokens of each sequence over all its T_b = seq_lens[b]
  * tokens, whose K and V the cache already holds: row i of sequence b sees tokens
- * 0 .. T_b - n_b + i. A row that sees none (T_b < n_b) yields zeros. */
+ * 0 .. T_b - n_b + i. A row that sees none (T_b < n_b) yields zeros. An int8 value is
+ * its product with its scale, unrounded; bf16 rows and q are rounded to fp16 first, as
+ * in pa_decode (magnitudes above 65504 become infinities). */
 int pa_prefill(const pa_prefill_args *args, void *stream);
 
 /* Differential attention of the same rows. Query heads 2 i and 2 i + 1 are the two

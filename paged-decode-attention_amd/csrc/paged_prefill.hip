@@ -16,22 +16,31 @@
 // is a row of its own in the kernel; neighbouring waves hold the two maps of the
 // same rows and meet once, at the end.
 //
-// A workgroup of four waves takes 128 rows, 32 a wave. K and V of a tile of
-// tokens go through registers (where 1-byte and bf16 caches become the fp16
-// values that the decode attends over) into LDS, double-buffered: the next
-// tile's loads are in flight while this one is computed.
+// A workgroup takes 32 rows a wave, 128 or 256 in all. K and V of a tile of tokens go
+// through registers (where 1-byte and bf16 caches become fp16; int8 values exactly,
+// their scales meet the scores and P) into LDS, double-buffered: the next tile's loads
+// are in flight while this one is computed.
 //   S^T[tok, row] = K . Q^T     v_mfma_f32_32x32x16_f16, a lane's column is its row
 //   O^T[d, row]  += V^T . P^T   the same; P^T comes straight from the S
 //                               accumulators, V^T from LDS by transposing reads
 // The softmax runs in the log2 domain over one pass; the running maximum moves
-// only when a tile exceeds it by kRescaleLog2, which keeps P below 2^8 and
-// leaves most tiles without a rescale. P is rounded to fp16 for its product
-// (half a unit in 2^-11, the same rounding as the cache's rows); scores,
-// maxima, sums and outputs stay in fp32 until the one rounding of the result.
+// only when a tile exceeds it by kRescaleLog2, which leaves most tiles without a
+// rescale. P is rounded to fp16 for its product (half a step of 2^-10: 1.3 times the
+// error that the result's own rounding makes, see the streams for two products);
+// scores, maxima, sums and outputs stay in fp32 until the one rounding of the result.
+//
+// What bounds it: a long prompt the card's power (16,384 tokens, 32 q / 8 kv heads of
+// 128, fp16: 2,210-2,300 us, 960-990 TFLOP/s; with all inputs zero 1,855, and a library
+// product of 8192^3 runs at 1,140-1,350 on data, 1,810 on zeros); in between, the
+// softmax's VALU instructions, about as long as the products that they alternate with;
+// small launches the latency of the chain length -> page -> K. Tried and slower or equal:
+// K a tile ahead of V with its products between the softmax's instructions, three
+// waves a SIMD on 32-token tiles, s_setprio around the products, block-table entries in
+// lanes instead of scalar loads.
 //
 // Where rows are few and sequences long, the tokens are cut into num_splits
 // chunks; each writes a normalised fp32 partial and its log2-sum-exp, and a
-// second kernel joins them.
+// second kernel joins them. Fewer rows still: paged_stream.hip.
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -774,7 +783,7 @@ int attend(const pa_prefill_args *a, int maps, void *stream) {
   PParams p;
   const int rc = build(a, maps, &p);
   if (rc != PA_OK) return rc;
-  if (p.tiles == 0 || p.num_tokens == 0) return pa_ok();
+  if (p.batch == 0 || p.num_tokens == 0) return pa_ok();  // (the searches need a sequence)
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int d = a->head_dim;
   hipError_t e;

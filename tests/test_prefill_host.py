@@ -125,6 +125,9 @@ def test_c_refusals_of_one_form():
                        ({"num_q_heads": 9, "num_kv_heads": 3}, INVALID)):
         assert lib.pa_diff_prefill(ctypes.byref(_args(True, **over)), None) == code, over
     assert lib.pa_prefill(ctypes.byref(_args(head_dim=256)), None) == _abi.PA_OK
+    # rows of no sequence: nothing to do (before any HIP call)
+    for form in (_abi.PA_FORM_TILES, _abi.PA_FORM_STREAMS, _abi.PA_FORM_STREAMS16):
+        assert lib.pa_prefill(ctypes.byref(_args(batch=0, num_tokens=500, form=form)), None) == _abi.PA_OK
 
 
 def _table_args(**over):
