@@ -369,8 +369,10 @@ typedef struct pa_prefill_args {
   int32_t num_blocks; /* pool size; block-table entries are clamped into it */
   int32_t max_blocks; /* block_table row length */
   int32_t num_splits; /* >= 1; > 1 cuts every row tile's tokens into at most that many chunks */
-  int32_t max_seq_len; /* > 0: chunks no shorter than those of a sequence this long, so a
-                          ragged batch's short sequences take few; 0: each its own */
+  int32_t chunks;      /* > 0: chunks that all row tiles of a kv head (pair) are cut into
+                          together, about: by the lengths the launch finds, so a ragged
+                          batch's long sequences take many and its short ones few. 0:
+                          every row tile is cut into num_splits, whatever the others */
   int32_t form;        /* PA_FORM_* */
   int64_t stride_qt, stride_qh;            /* element strides (token, head) */
   int64_t stride_kn, stride_kt, stride_kh; /* shared by k_cache and v_cache */

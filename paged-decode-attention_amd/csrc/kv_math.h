@@ -1,6 +1,7 @@
 // The stored forms of a KV cache as fp16 operands, and the loads of its pages:
-// shared by the attention kernels of this library, so that every one of them
-// attends over the same values.
+// shared by the attention kernels of this library. (int8: the decode rounds the
+// product with the scale to fp16, the prompt kernels take the values as they are and
+// their scales in fp32.)
 #ifndef PA_KV_MATH_H_
 #define PA_KV_MATH_H_
 

@@ -336,23 +336,6 @@ __device__ __forceinline__ void add_wild(RowState<D, W> &st, const uint8_t *v, i
   }
 }
 
-// The sum over the wave, in every lane (all lanes active): adds across a row of 16
-// lanes by DPP, then of the rows' last lanes into the next rows.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_add(int x) {
-  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
-}
-
-__device__ __forceinline__ int wave_sum(int x) {
-  x = dpp_add<0x111, 0xf>(x);  // row_shr:1
-  x = dpp_add<0x112, 0xf>(x);
-  x = dpp_add<0x114, 0xf>(x);
-  x = dpp_add<0x118, 0xf>(x);
-  x = dpp_add<0x142, 0xa>(x);  // row_bcast:15 into rows 1 and 3
-  x = dpp_add<0x143, 0xc>(x);  // row_bcast:31 into rows 2 and 3
-  return __builtin_amdgcn_readlane(x, 63);
-}
-
 // The row tile of this rank, longest first: a launch of a few rounds of workgroups
 // otherwise ends with whatever long tiles come last, alone on their CUs. Tile i of
 // sequence b sees about o_b + i row tiles' worth of tokens, o_b those before its new
@@ -440,7 +423,7 @@ paged_prefill_kernel(const PParams p) {
   int lo = 0, hi = rt.hi;
   bool direct = true;  // the row tile is this workgroup's alone: no partials
   if (p.num_splits > 1) {
-    const int chunk = split_tokens<kSplitUnit>(p, rt.hi);
+    const int chunk = split_tokens(p, rt.hi, split_units<G::kRowTile>(p, lane));
     if (split > 0 && (int64_t)split * chunk >= rt.hi) return;  // empty
     lo = split * chunk;
     hi = min(rt.hi, lo + chunk);
@@ -648,7 +631,7 @@ int build(const pa_prefill_args *a, int maps, PParams *out) {
     return pa_fail(PA_ERR_INVALID, "num_splits %d not in [1, %d]", a->num_splits, PA_MAX_SPLITS);
   if (a->num_splits > 1 && (!a->part_out || !a->part_lse))
     return pa_fail(PA_ERR_INVALID, "num_splits %d needs part_out and part_lse", a->num_splits);
-  if (a->max_seq_len < 0) return pa_fail(PA_ERR_INVALID, "max_seq_len %d < 0", a->max_seq_len);
+  if (a->chunks < 0) return pa_fail(PA_ERR_INVALID, "chunks %d < 0", a->chunks);
   if (a->form < PA_FORM_TILES || a->form > PA_FORM_STREAMS16) return pa_fail(PA_ERR_INVALID, "form %d unknown", a->form);
   if (!a->query_start_loc && a->num_tokens != a->batch)
     return pa_fail(PA_ERR_INVALID, "without query_start_loc num_tokens (%d) must be batch (%d)", a->num_tokens, a->batch);
@@ -696,12 +679,16 @@ int build(const pa_prefill_args *a, int maps, PParams *out) {
   const int group = a->num_q_heads / a->num_kv_heads;
   const int units = a->num_kv_heads / maps;
   if ((int64_t)a->num_tokens * a->num_q_heads >= 2 * gib) return pa_fail(PA_ERR_UNSUPPORTED, "num_tokens * num_q_heads must be below 2^31");
-  const int columns = a->form == PA_FORM_TILES ? kRowsPerWave * (d * maps >= 128 && d < 256 ? 8 : 4) : a->form == PA_FORM_STREAMS ? 32 : 16;
+  const int waves = a->form == PA_FORM_TILES && d * maps >= 128 && d < 256 ? 8 : kWaves;
+  const int columns = a->form == PA_FORM_TILES ? kRowsPerWave * waves : a->form == PA_FORM_STREAMS ? 32 : 16;
   const int row_tile = columns / maps;
   const int seq_tiles = (group + row_tile - 1) / row_tile;
   const int64_t tiles = a->query_start_loc ? (int64_t)a->num_tokens * group / row_tile + a->batch
                                            : (int64_t)a->batch * seq_tiles;
-  if (tiles * units * a->num_splits >= 2 * gib) return pa_fail(PA_ERR_UNSUPPORTED, "too many workgroups");
+  // a launch holds fewer than 2^32 threads (the merge: a wave an output row)
+  if (tiles * units >= 2 * gib || tiles * units * a->num_splits * waves >= 4 * gib / 64 ||
+      (a->num_splits > 1 && (int64_t)a->num_tokens * (a->num_q_heads / maps) >= 4 * gib / 64 - 4))
+    return pa_fail(PA_ERR_UNSUPPORTED, "too many rows and splits for one launch: 2^26 waves at most");
 
   PParams p = {};
   p.q = static_cast<const uint8_t *>(a->q);
@@ -726,7 +713,7 @@ int build(const pa_prefill_args *a, int maps, PParams *out) {
   p.max_tokens = a->max_blocks * bs;
   p.log2_page = __builtin_ctz((unsigned)bs);
   p.num_splits = a->num_splits;
-  p.max_seq_len = std::min(a->max_seq_len, p.max_tokens);
+  p.chunks = std::min(a->chunks, 1 << 30);
   p.tiles = (int32_t)tiles;
   p.sqt = (int32_t)a->stride_qt;
   p.sqh = (int32_t)a->stride_qh;

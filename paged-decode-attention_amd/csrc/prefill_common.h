@@ -7,6 +7,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "kv_math.h"
 #include "launch_math.h"
 #include "pa_errors.h"
@@ -29,7 +31,7 @@ struct PParams {
   const float *norm;     // differential: [DV] or NULL
   int32_t batch, num_tokens, units, group, num_q_heads;
   int32_t num_blocks, max_tokens, log2_page, num_splits;
-  int32_t max_seq_len;   // > 0: chunks no shorter than those of a sequence this long
+  int32_t chunks;        // > 0: chunks wanted of all row tiles of a unit together
   int32_t tiles;         // row tiles of the launch
   int32_t sqt, sqh, sot, soh;  // elements
   uint32_t skn, skt, skh, ssn, sst;  // bytes
@@ -61,6 +63,32 @@ constexpr int kSplitUnit = 128;  // splits are multiples of this many tokens
 // the load returns zeros.
 constexpr uint32_t kOutside = 0xfffffff0u;
 constexpr int kRsrcBytes = (int)kOutside;
+
+// x with what DPP control CTRL hands the lanes of ROWS (the others: `none`).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp(int x, int none) {
+  return __builtin_amdgcn_update_dpp(none, x, CTRL, ROWS, 0xf, false);
+}
+
+// The wave's lanes combined, for every lane; `none` changes nothing.
+template <typename OP>
+__device__ __forceinline__ int wave_join(int x, int none, OP op) {
+  x = op(x, dpp<0x111, 0xf>(x, none));  // row_shr:1
+  x = op(x, dpp<0x112, 0xf>(x, none));
+  x = op(x, dpp<0x114, 0xf>(x, none));
+  x = op(x, dpp<0x118, 0xf>(x, none));
+  x = op(x, dpp<0x142, 0xa>(x, none));  // row_bcast:15 into rows 1 and 3
+  x = op(x, dpp<0x143, 0xc>(x, none));  // row_bcast:31 into rows 2 and 3
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
+__device__ __forceinline__ int wave_sum(int x) {
+  return wave_join(x, 0, [](int a, int b) { return a + b; });
+}
+
+__device__ __forceinline__ int wave_max(int x) {
+  return wave_join(x, INT32_MIN, [](int a, int b) { return max(a, b); });
+}
 
 // x combined with the value of the other half of the wave (lane ^ 32).
 __device__ __forceinline__ float half_max(float x) {
@@ -193,13 +221,35 @@ __device__ __forceinline__ RowTile tile_at(const PParams &p, int b, int index) {
   return t;
 }
 
-// Tokens of a split of a row tile that sees `hi`, a multiple of UNIT: the tile's own
-// chunk, or that of a tile that sees max_seq_len if it is larger (ragged batches:
-// long sequences take all splits, short ones few).
-template <int UNIT>
-__device__ __forceinline__ int split_tokens(const PParams &p, int hi) {
-  const uint32_t units = ((uint32_t)max(hi, p.max_seq_len) + UNIT - 1) / UNIT;
-  return (int)div_by(units + p.num_splits - 1, p.by_splits) * UNIT;
+// The most units of a split (kSplitUnit tokens each) with p.chunks: the num_splits'th
+// part of the longest sequence, and what gives p.chunks over all row tiles of ROWS
+// rows together, so a ragged batch's long sequences take many and its short ones one.
+// Every workgroup sums the lengths itself, two loads a lane for 64 sequences, and the
+// merge comes to the same. 0 without p.chunks.
+template <int ROWS>
+__device__ __forceinline__ uint32_t split_units(const PParams &p, int lane) {
+  if (p.chunks == 0) return 0;
+  int longest = 0, total = 0;  // total: units; a lane's stops at 2^24
+  for (int b = lane; b < p.batch; b += 64) {
+    const int n = p.start ? max(row_start(p, b + 1) - row_start(p, b), 0) : 1;
+    if (n == 0) continue;
+    const int len = max(0, min(ro(p.seq_lens)[b], p.max_tokens));
+    longest = max(longest, len);
+    const uint32_t tiles = ((uint32_t)(n * p.group) + ROWS - 1) / ROWS;
+    const uint32_t units = (uint32_t)(max(len - n / 2, 0) + kSplitUnit - 1) / kSplitUnit;
+    total = (int)min((uint64_t)total + (uint64_t)tiles * units, (uint64_t)1 << 24);
+  }
+  const uint32_t most = div_by(((uint32_t)wave_max(longest) + kSplitUnit - 1) / kSplitUnit + p.num_splits - 1, p.by_splits);
+  return max(max(most, ((uint32_t)wave_sum(total) + p.chunks - 1) / p.chunks), 1u);
+}
+
+// Tokens of a split of a row tile that sees `hi`: equal shares of at most `most`
+// units, or (0) the num_splits'th part.
+__device__ __forceinline__ int split_tokens(const PParams &p, int hi, uint32_t most) {
+  const uint32_t units = ((uint32_t)hi + kSplitUnit - 1) / kSplitUnit;
+  if (most == 0) return (int)div_by(units + p.num_splits - 1, p.by_splits) * kSplitUnit;
+  const uint32_t pieces = max((units + most - 1) / most, 1u);
+  return (int)((units + pieces - 1) / pieces) * kSplitUnit;
 }
 
 template <int POLICY, int WORDS>
@@ -324,7 +374,10 @@ __device__ __forceinline__ void store_partial(const PParams &p, GET get, float m
 }
 
 // Joins the partials of a split launch: one wave an output row, W / 64 elements a
-// lane (W = 32: the upper half of the wave idles). Row tiles of one split are done;
+// lane (W = 32: the upper half of the wave idles), up to four splits' loads at once.
+// Bound by latency for few rows (5 us), by the partials' bytes for many (25,700 rows of
+// two maps and 128 elements, two splits: 14 us). Several rows a wave, or weights found
+// one a lane, took 18-21 us there. Row tiles of one split are done;
 // empty splits were not written and are not read.
 template <int W, int MAPS, int ROWS>
 __global__ void __launch_bounds__(256) prefill_merge_kernel(const PParams p) {
@@ -345,39 +398,67 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(const PParams p) {
   const int token = packed - row_start(p, b);
   const int in_group = out_head % p.group;
   const RowTile rt = tile_at<ROWS>(p, b, (token * p.group + in_group) / ROWS);
-  const int chunk = split_tokens<kSplitUnit>(p, rt.hi);
+  const int chunk = split_tokens(p, rt.hi, split_units<ROWS>(p, lane));
   if (rt.hi <= chunk) return;  // written by its one workgroup
   const int n = (rt.hi - 1) / chunk + 1;
   const bool sees = rt.first + token >= 0;
 
-  float y[E] = {};
   const int d0 = E * lane;
   const bool mine = d0 < W;
+  const int64_t at = (int64_t)packed * p.num_q_heads + MAPS * out_head;
+  const int64_t step = (int64_t)p.num_tokens * p.num_q_heads;
+  float m[MAPS], sum[MAPS] = {}, acc[MAPS][E] = {};
+#pragma unroll
+  for (int map = 0; map < MAPS; ++map) m[map] = -INFINITY;
+  // `ahead` splits, their loads on the way together; one that saw nothing of the row
+  // (-inf) is left out whatever it holds
+  auto join = [&](int s, auto ahead) {
+    constexpr int kAhead = decltype(ahead)::value;
+    float lse[kAhead][MAPS], o[kAhead][MAPS][E] = {};
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+      for (int map = 0; map < MAPS; ++map) {
+        lse[i][map] = p.part_lse[at + map + (s + i) * step];
+        if (mine) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[i][map][e] = p.part_out[(at + map + (s + i) * step) * W + d0 + e];
+        }
+      }
+#pragma unroll
+    for (int map = 0; map < MAPS; ++map) {
+      float top = m[map];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) top = fmaxf(top, lse[i][map]);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float old = __builtin_amdgcn_exp2f(m[map] - base);
+      sum[map] *= old;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[map][e] *= old;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const float w = __builtin_amdgcn_exp2f(lse[i][map] - base);
+        sum[map] += w;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[map][e] += lse[i][map] == -INFINITY ? 0.f : w * o[i][map][e];
+      }
+      m[map] = top;
+    }
+  };
+  int s = 0;
+  for (; s + 4 <= n; s += 4) join(s, std::integral_constant<int, 4>());
+  if (s + 2 <= n) {
+    join(s, std::integral_constant<int, 2>());
+    s += 2;
+  }
+  if (s < n) join(s, std::integral_constant<int, 1>());
+  float y[E] = {};
 #pragma unroll
   for (int map = 0; map < MAPS; ++map) {
-    const int64_t at = (int64_t)packed * p.num_q_heads + MAPS * out_head + map;
-    const int64_t step = (int64_t)p.num_tokens * p.num_q_heads;
-    float m = -INFINITY, sum = 0.f, acc[E] = {};
-    for (int s = 0; s < n; ++s) {
-      const float lse = p.part_lse[at + s * step];
-      float o[E] = {};
-      if (mine) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = p.part_out[(at + s * step) * W + d0 + e];
-      }
-      if (lse == -INFINITY) continue;
-      const float m_new = lse > m ? lse : m;
-      const float old = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
-      const float w = __builtin_amdgcn_exp2f(lse - m_new);
-      sum = sum * old + w;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = acc[e] * old + w * o[e];
-      m = m_new;
-    }
-    const float inv = sees ? 1.0f / sum : 0.f;
+    const float inv = sees ? 1.0f / sum[map] : 0.f;
     const float f = map == 1 ? -inv * p.lam[(int64_t)out_head * p.slam] : inv;
 #pragma unroll
-    for (int e = 0; e < E; ++e) y[e] += acc[e] * f;
+    for (int e = 0; e < E; ++e) y[e] += acc[map][e] * f;
   }
   if constexpr (MAPS == 2) {
     if (p.norm) {

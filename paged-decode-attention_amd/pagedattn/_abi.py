@@ -190,7 +190,7 @@ class PaPrefillArgs(ctypes.Structure):
         ("num_blocks", _i32),
         ("max_blocks", _i32),
         ("num_splits", _i32),
-        ("max_seq_len", _i32),
+        ("chunks", _i32),
         ("form", _i32),
         ("stride_qt", _i64),
         ("stride_qh", _i64),

@@ -30,15 +30,18 @@ _PER_CU = {_abi.PA_FORM_TILES: {256: 1, 128: 1}, _abi.PA_FORM_STREAMS: {256: 1},
 # A split is a multiple of this many tokens; fewer than MIN_SPLIT_TOKENS are not
 # worth a partial and its share of the merge.
 MIN_SPLIT_TOKENS = 256
+# How many times the average sequence's chunks the longest may take.
+UNEVEN = {_abi.PA_FORM_TILES: 1, _abi.PA_FORM_STREAMS: 3, _abi.PA_FORM_STREAMS16: 3}
 # Launches with less than this share of the chip's workgroups are split.
 SPLIT_BELOW = 0.85
 
 
 def _plan(rows: int, batch: int, units: int, longest: int, cus: int, width: int, maps: int) -> tuple[int, int]:
-    """(form, num_splits) from shapes alone: `rows` (token, head) rows in all for
-    each of `units` kv heads (pairs of them in the differential forms), cache rows
+    """(form, num_splits) from shapes alone: `rows` (token, head) rows in all
+    for each of `units` kv heads (pairs of them in the differential forms), cache rows
     of `width` elements. Sequences whose rows a stream's columns hold on average
-    stream; the splits fill the chip once."""
+    stream. Splits fill the chip (`_chunks`), and a sequence longer than the average may
+    take more of them than its share."""
     form = _abi.PA_FORM_TILES
     for few in (_abi.PA_FORM_STREAMS16, _abi.PA_FORM_STREAMS):
         if rows * maps <= _COLUMNS[few] * batch:
@@ -51,8 +54,19 @@ def _plan(rows: int, batch: int, units: int, longest: int, cus: int, width: int,
     slots = _PER_CU[form].get(width, 2) * cus
     splits = 1
     if work < SPLIT_BELOW * slots:
-        splits = max(1, min(-(-slots // work), -(-longest // MIN_SPLIT_TOKENS), _abi.PA_MAX_SPLITS))
+        uneven = min(batch, UNEVEN[form])
+        splits = max(1, min(-(-slots // work) * uneven, -(-longest // MIN_SPLIT_TOKENS), _abi.PA_MAX_SPLITS))
     return form, splits
+
+
+def _chunks(form: int, units: int, cus: int, width: int) -> int:
+    """Chunks of a split launch for each unit; 0: every tile by itself. They fill 3/4 of
+    the chip: a sequence's chunks are more than its share by half a one on average, and
+    a few more than the chip holds take a round of their own (24 int8 sequences of up to
+    8,000 tokens, 5 new: 0.6 67 us, 0.75 63, 0.8 76). (Tiles' chunks come longest first, which balances as well, and
+    sizing them by the batch's lengths gave more partials: 12 prompts of 60 to 700
+    tokens after up to 3,000, pairs of 64-element heads, 86 against 96 us.)"""
+    return 0 if form == _abi.PA_FORM_TILES else max(1, _PER_CU[form].get(width, 2) * cus * 3 // (4 * units))
 
 
 # Checked argument structs by the geometry they were checked for: shapes, strides,
@@ -184,12 +198,14 @@ def _check(maps, q, cache, start, out, sm_scale, num_splits, max_seq_len, lam, n
     capacity = blocks * cache.block_size
     longest = capacity if max_seq_len is None else max(0, min(max_seq_len, capacity))
     form, planned = _plan(n * (hq // hkv), b, hkv // maps, longest, _cu_count(q.device), maps * d, maps)
-    num_splits = planned if num_splits is None else num_splits
+    chunks = 0
+    if num_splits is None:
+        num_splits, chunks = planned, _chunks(form, hkv // maps, _cu_count(q.device), maps * d)
     rows = num_splits * n * hq if num_splits > 1 else 0
     args = _abi.PaPrefillArgs()
     args.batch, args.num_tokens, args.num_q_heads, args.num_kv_heads, args.head_dim = b, n, hq, hkv, d
     args.block_size, args.num_blocks, args.max_blocks = cache.block_size, k.shape[0], blocks
-    args.num_splits, args.max_seq_len, args.form = num_splits, 0 if max_seq_len is None else longest, form
+    args.num_splits, args.chunks, args.form = num_splits, chunks, form
     args.stride_qt, args.stride_qh = qst[0], qst[1]
     args.stride_kn, args.stride_kt, args.stride_kh = kst[0], kst[1], kst[2]
     args.stride_sn, args.stride_st = sst[0], sst[1]
@@ -219,12 +235,12 @@ def paged_prefill_hip(
     row i of n_b sees tokens 0 .. T_b - n_b + i. A row that sees none is zeros.
     Rows of no sequence (padding behind the last) are left as they are in `out`.
 
-    `num_splits` cuts each row tile's tokens into at most that many chunks, joined
-    by a second kernel; None plans it from the shapes alone, with no device sync.
-    `max_seq_len` (a host int; None: what the block table can hold) is what it
-    plans by, and, if given, sizes every chunk as of a sequence that long, so a
-    ragged batch's short sequences are cut less. Results do not depend on it
-    beyond rounding, and longer sequences are attended whole.
+    `num_splits` cuts the longest sequence's tokens into at most that many chunks, and
+    the others' into chunks no longer, joined by a second kernel. None plans them from
+    the shapes alone, with no device sync: the kernel itself sizes the chunks by the
+    lengths it finds, so that they fill the chip evenly. `max_seq_len` (a host int;
+    None: what the block table can hold) is what that plans by. Results do not depend
+    on either beyond rounding, and longer sequences are attended whole.
     """
     return _attend("pa_prefill", 1, q, cache, query_start_loc, out, sm_scale, num_splits, max_seq_len)
 

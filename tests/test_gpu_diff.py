@@ -77,6 +77,15 @@ def test_splits(splits, new):
         check(q, c, start, lam, w, num_splits=splits, max_seq_len=1200)
 
 
+def test_ragged_splits():
+    """Planned splits, sized by the lengths that the launch finds."""
+    total = [0, 3000, 5, 40, 1, 700] + [30] * 70
+    q, c, start = case(QWEN25_05B, [1] * len(total), total, "int8", torch.float32, page=32, seed=29)
+    lam, w = weights(QWEN25_05B, 29)
+    check(q, c, start, lam, w)
+    check(q, c, start, lam, w, max_seq_len=3000)
+
+
 @pytest.mark.parametrize("splits", [1, 3])
 def test_empty_rows_and_sequences(splits):
     q, c, start = case(QWEN25_05B, [1, 1, 1], [0, 40, 0], seed=23)

@@ -132,6 +132,20 @@ def test_splits(shape, splits, longest):
     check(q, c, start, num_splits=splits, max_seq_len=longest)
 
 
+@pytest.mark.parametrize("batch", [2, 9, 70])
+@pytest.mark.parametrize("long", [900, 5000])
+def test_ragged_splits(batch, long):
+    """Planned splits, sized by the lengths that the launch finds: one long sequence among short and
+    empty ones, then another as long, all with the same plan."""
+    total = [long if i == 1 else 17 * (i % 6) for i in range(batch)]
+    new = [min(1 + i % 3, n) for i, n in enumerate(total)]
+    q, c, start = case(QWEN25_05B, new, total, seed=23)
+    check(q, c, start, max_seq_len=long)
+    c.seq_lens[1] = long // 3
+    check(q, c, start, max_seq_len=long)
+    check(q, c, start, max_seq_len=300)  # shorter than the longest: attended whole all the same
+
+
 @pytest.mark.parametrize("batch", [63, 64, 65, 130, 4200])
 def test_many_sequences(batch):
     """The search for a tile's sequence, at one, two and three rounds of 64 probes."""
@@ -270,7 +284,7 @@ def test_pool_past_4_gib():
     assert torch.equal(paged_prefill_hip(q, big, offsets(start)), want)
 
 
-@pytest.mark.parametrize("splits", [1, 4])
+@pytest.mark.parametrize("splits", [1, 4, None])
 def test_graph_replays_follow_the_lengths(splits):
     """Captured once, replayed with other lengths, offsets and q between eager work."""
     q, c, start = case(LLAMA3_8B, [5, 9], [90, 40], seed=15, pad=2)

@@ -82,7 +82,7 @@ BAD = [
     ({"block_size": 48}, UNSUPPORTED), ({"block_size": 512}, UNSUPPORTED), ({"kv_dtype": 7}, INVALID),
     ({"io_dtype": 2}, INVALID), ({"sm_scale": 0.0}, INVALID), ({"sm_scale": -1.0}, INVALID),
     ({"sm_scale": NAN}, INVALID), ({"sm_scale": INF}, INVALID), ({"num_splits": 0}, INVALID),
-    ({"num_splits": 5000}, INVALID), ({"num_splits": 2}, INVALID), ({"max_seq_len": -1}, INVALID),
+    ({"num_splits": 5000}, INVALID), ({"num_splits": 2}, INVALID), ({"chunks": -1}, INVALID),
     ({"form": 3}, INVALID), ({"form": -1}, INVALID), ({"stride_qt": -8}, INVALID), ({"stride_kn": -8}, INVALID),
     ({"stride_btb": -1}, INVALID), ({"q": FAKE + 8}, INVALID), ({"stride_qh": 132}, INVALID),
     ({"out": FAKE + 2}, INVALID), ({"stride_oh": 129}, INVALID), ({"k_cache": FAKE + 4}, INVALID),
@@ -95,6 +95,8 @@ BAD = [
     ({"stride_qt": 1 << 31}, UNSUPPORTED), ({"stride_ot": 1 << 31}, UNSUPPORTED),
     ({"num_tokens": 1 << 26}, UNSUPPORTED),
     ({"num_tokens": 1 << 25, "num_splits": 4096, "part_out": FAKE, "part_lse": FAKE}, UNSUPPORTED),
+    ({"num_tokens": 1 << 24, "num_splits": 2, "part_out": FAKE, "part_lse": FAKE}, UNSUPPORTED),
+    ({"num_tokens": 1 << 23, "num_splits": 64, "part_out": FAKE, "part_lse": FAKE}, UNSUPPORTED),
     ({"num_splits": 2, "part_out": FAKE + 4, "part_lse": FAKE}, INVALID),
 ]
 
