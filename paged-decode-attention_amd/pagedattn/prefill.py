@@ -87,17 +87,18 @@ def _attend(fn_name, maps, q, cache, start, out, sm_scale, num_splits, max_seq_l
     # (numbers by value: a tensor given as one would be a key by its identity)
     sm_scale = None if sm_scale is None else float(sm_scale)
     num_splits = None if num_splits is None else int(num_splits)
-    max_seq_len = None if max_seq_len is None else int(max_seq_len)
+    # (the plan's unit, so a serving loop's growing length is not a geometry every step)
+    longest = None if max_seq_len is None else max(0, -(-int(max_seq_len) // MIN_SPLIT_TOKENS)) * MIN_SPLIT_TOKENS
     norm_eps, out_scale = float(norm_eps), float(out_scale)
     key = (fn_name, q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(),
            v.shape, v.stride(), v.dtype, v.get_device(), bt.shape, bt.stride(), bt.dtype, bt.get_device(),
            sl.shape, sl.stride(), sl.dtype, sl.get_device(), cache.kv_dtype, cache.block_size, shape.num_q_heads,
-           shape.num_kv_heads, shape.head_dim, sm_scale, num_splits, max_seq_len, norm_eps, out_scale)
+           shape.num_kv_heads, shape.head_dim, sm_scale, num_splits, longest, norm_eps, out_scale)
     for t in (start, out, lam, norm_weight, ks, vs):
         key += (None,) if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
     hit = _CHECKED.get(key)
     if hit is None:
-        hit = _check(maps, q, cache, start, out, sm_scale, num_splits, max_seq_len, lam, norm_weight, norm_eps,
+        hit = _check(maps, q, cache, start, out, sm_scale, num_splits, longest, lam, norm_weight, norm_eps,
                      out_scale)
         if len(_CHECKED) >= _CHECKED_MAX:
             _CHECKED.clear()
@@ -128,7 +129,7 @@ def _attend(fn_name, maps, q, cache, start, out, sm_scale, num_splits, max_seq_l
     return out
 
 
-def _check(maps, q, cache, start, out, sm_scale, num_splits, max_seq_len, lam, norm_weight, norm_eps, out_scale):
+def _check(maps, q, cache, start, out, sm_scale, num_splits, longest, lam, norm_weight, norm_eps, out_scale):
     """(struct without pointers or None where there are no rows, the result's shape,
     bytes of part_out, floats of all partials) of a call, or the error of a wrong one."""
     if q.dim() != 3:
@@ -196,7 +197,7 @@ def _check(maps, q, cache, start, out, sm_scale, num_splits, max_seq_len, lam, n
     if n == 0 or b == 0:
         return None, out_shape, 0, 0
     capacity = blocks * cache.block_size
-    longest = capacity if max_seq_len is None else max(0, min(max_seq_len, capacity))
+    longest = capacity if longest is None else min(longest, capacity)
     form, planned = _plan(n * (hq // hkv), b, hkv // maps, longest, _cu_count(q.device), maps * d, maps)
     chunks = 0
     if num_splits is None:
